@@ -34,6 +34,8 @@ EXPORTS = [
     "issm_hilbert_codes", "issm_hilbert_order", "issm_transpose_states", "issm_layer_params", "issm_linear_fwd", "issm_linear_dx", "issm_linear_dw", "issm_linear_dw_pair", "issm_linear_dw_scratch_bytes", "issm_layer_out", "issm_layer_in",
     "issm_param_gen_fwd_only", "issm_conv_param_gen_fwd", "issm_layer_end", "issm_box_dist_fwd_only",
     "issm_box_table", "issm_box_table_bwd",
+    "issm_gated_scan_saved_bytes", "issm_gated_scan_workspace_bytes", "issm_gated_scan_fwd", "issm_gated_scan_bwd", "issm_gated_scan_step",
+    "issm_rotary", "issm_rotary_norm_fwd", "issm_rotary_norm_bwd_bytes", "issm_rotary_norm_bwd",
     "issm_pn2_furthest_point_sampling", "issm_pn2_ball_query", "issm_pn2_group_points", "issm_pn2_group_points_grad",
     "issm_pn2_gather_points", "issm_pn2_gather_points_grad", "issm_pn2_three_nn", "issm_pn2_three_interpolate",
     "issm_pn2_three_interpolate_grad", "issm_pn2_group_xyz_points", "issm_pn2_group_points_grad_rows",
@@ -153,6 +155,41 @@ class TransposeArgs(C.Structure):
     ]
 
 
+class GatedScanArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("channels", C.c_int32), ("dtype", C.c_int32), ("flags", C.c_uint32),
+        ("x", C.c_void_p), ("gate", C.c_void_p), ("in_gate", C.c_void_p),
+        ("x_stride", C.c_int64 * 2), ("gate_stride", C.c_int64 * 2), ("in_gate_stride", C.c_int64 * 2),
+        ("A", C.c_void_p), ("h0", C.c_void_p), ("seq_idx", C.c_void_p), ("seq_idx_stride", C.c_int64 * 2),
+        ("y", C.c_void_p), ("last", C.c_void_p), ("saved", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64 * 2), ("dlast", C.c_void_p),
+        ("dx", C.c_void_p), ("dgate", C.c_void_p), ("din_gate", C.c_void_p), ("dA", C.c_void_p), ("dh0", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
+    ]
+
+
+class GatedScanStepArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int32), ("channels", C.c_int32), ("slots", C.c_int64), ("dtype", C.c_int32), ("flags", C.c_uint32),
+        ("x", C.c_void_p), ("gate", C.c_void_p), ("in_gate", C.c_void_p),
+        ("x_stride", C.c_int64), ("gate_stride", C.c_int64), ("in_gate_stride", C.c_int64),
+        ("A", C.c_void_p), ("state", C.c_void_p), ("state_stride", C.c_int64), ("slots_of", C.c_void_p), ("slots_64", C.c_int32), ("y", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("headdim", C.c_int32), ("rot", C.c_int32), ("heads", C.c_int32 * 2),
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("flags", C.c_uint32), ("eps", C.c_float),
+        ("x", C.c_void_p * 2), ("x_stride", (C.c_int64 * 3) * 2), ("w", C.c_void_p * 2), ("y", C.c_void_p * 2),
+        ("table", C.c_void_p), ("table_rows", C.c_int64), ("positions", C.c_void_p), ("positions_stride", C.c_int64 * 2),
+        ("positions_64", C.c_int32),
+        ("dy", C.c_void_p * 2), ("dy_stride", (C.c_int64 * 3) * 2), ("dx", C.c_void_p * 2), ("dw", C.c_void_p * 2),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t), ("stream", C.c_void_p),
+    ]
+
+
 class HilbertArgs(C.Structure):
     _fields_ = [
         ("batch", C.c_int32), ("npoint", C.c_int32), ("bits", C.c_int32), ("order", C.c_int32 * 3),
@@ -250,6 +287,16 @@ def load() -> C.CDLL:
     lib.issm_box_table_bwd.argtypes = [P(BoxTableArgs), vp, vp, vp, vp]   # (without: addresses arrive as 32-bit integers)
     lib.issm_linear_dw_scratch_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
     lib.issm_linear_dw_scratch_bytes.restype = C.c_size_t
+    PS = P(C.c_size_t)
+    lib.issm_gated_scan_saved_bytes.argtypes = [P(GatedScanArgs), PS]
+    lib.issm_gated_scan_workspace_bytes.argtypes = [P(GatedScanArgs), C.c_int32, PS]
+    lib.issm_gated_scan_fwd.argtypes = [P(GatedScanArgs)]
+    lib.issm_gated_scan_bwd.argtypes = [P(GatedScanArgs)]
+    lib.issm_gated_scan_step.argtypes = [P(GatedScanStepArgs)]
+    lib.issm_rotary.argtypes = [P(RotaryArgs)]
+    lib.issm_rotary_norm_fwd.argtypes = [P(RotaryArgs)]
+    lib.issm_rotary_norm_bwd_bytes.argtypes = [P(RotaryArgs), PS]
+    lib.issm_rotary_norm_bwd.argtypes = [P(RotaryArgs)]
     _lib = lib
     return lib
 

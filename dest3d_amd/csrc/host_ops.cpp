@@ -1317,6 +1317,487 @@ std::vector<Tensor> scan_layer(const Tensor& in_key, const Tensor& in_query, con
   return linear_pair(core[0], out_key_proj, q, out_query_proj);
 }
 
+// ------------------------------------------------------------------------------------------------ gated linear recurrence
+// (a tensor that is the lazy negation of its memory is computed first)
+Tensor kernel_operand(const Tensor& t, at::ScalarType type) { return t.defined() ? io_cast(t.resolve_neg(), type) : t; }
+bool recorded(std::initializer_list<const Tensor*> inputs) {
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : inputs)
+      if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+void first_derivatives_only(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " has first derivatives only: its backward cannot be recorded (create_graph)");
+}
+
+struct GatedScan {
+  Tensor x, gate, in_gate, A, h0, seq;   // as the kernels read them
+  bool normalize = true, reverse = false;
+
+  static GatedScan make(const Tensor& x, const Tensor& gate, const Tensor& A, const Tensor& in_gate, const Tensor& h0, const Tensor& seq,
+                        bool normalize, bool reverse) {
+    GatedScan s;
+    const at::ScalarType io = kernel_type(x.scalar_type());
+    s.x = kernel_operand(x, io);
+    s.gate = kernel_operand(gate, io);
+    s.in_gate = kernel_operand(in_gate, io);
+    s.A = f32c(A.resolve_neg());
+    s.h0 = h0.defined() ? f32c(h0.resolve_neg()) : h0;
+    s.seq = cast(seq, at::kInt);
+    s.normalize = normalize;
+    s.reverse = reverse;
+    return s;
+  }
+  issm_gated_scan_args args() const {
+    issm_gated_scan_args a{};
+    a.batch = (int32_t)x.size(0);
+    a.seqlen = (int32_t)x.size(1);
+    a.channels = (int32_t)x.size(2);
+    a.dtype = code(x.scalar_type());
+    a.flags = (normalize ? ISSM_GS_NORMALIZE : 0u) | (reverse ? ISSM_GS_REVERSE : 0u);
+    auto strided = [](const Tensor& t, const void*& p, int64_t (&stride)[2]) {
+      p = data(t);
+      for (int i = 0; i < 2 && t.defined(); ++i) stride[i] = t.stride(i);
+    };
+    strided(x, a.x, a.x_stride);
+    strided(gate, a.gate, a.gate_stride);
+    strided(in_gate, a.in_gate, a.in_gate_stride);
+    a.A = data<const float>(A);
+    a.h0 = data<const float>(h0);
+    if (seq.defined()) {
+      a.seq_idx = data<const int32_t>(seq);
+      a.seq_idx_stride[0] = seq.stride(0);
+      a.seq_idx_stride[1] = seq.stride(1);
+    }
+    a.stream = stream_of(x);
+    return a;
+  }
+  bool empty() const { return x.numel() == 0; }
+  // (a row of no tokens ends in the state it starts from)
+  Tensor untouched() const { return h0.defined() ? h0.clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat)); }
+
+  struct Out {
+    Tensor y, last, saved;
+  };
+  Out forward(bool want_last, bool save) const {
+    Out o;
+    o.y = fresh(x.sizes(), x, x.scalar_type());
+    if (empty()) {
+      if (want_last) o.last = untouched();
+      return o;
+    }
+    issm_gated_scan_args a = args();
+    a.y = data(o.y);
+    if (want_last) {
+      o.last = fresh({x.size(0), x.size(2)}, x, at::kFloat);
+      a.last = data<float>(o.last);
+    }
+    if (save) {
+      size_t n = 0;
+      check(issm_gated_scan_saved_bytes(&a, &n), "issm_gated_scan_saved_bytes");
+      o.saved = fresh({(int64_t)n}, x, at::kByte);
+      a.saved = data(o.saved);
+    }
+    const Tensor ws = workspace(a, false);
+    check(issm_gated_scan_fwd(&a), "issm_gated_scan_fwd");
+    return o;
+  }
+  Tensor workspace(issm_gated_scan_args& a, bool back) const {
+    size_t n = 0;
+    check(issm_gated_scan_workspace_bytes(&a, back, &n), "issm_gated_scan_workspace_bytes");
+    if (!n) return Tensor();
+    const Tensor ws = fresh({(int64_t)n}, x, at::kByte);
+    a.workspace = data(ws);
+    a.workspace_bytes = n;
+    return ws;
+  }
+};
+
+// Inputs 0 .. 4 of the node: x, gate, A, in_gate, h0
+struct GatedScanFn : public Function<GatedScanFn> {
+  static constexpr int NIN = 5;
+  struct Record : torch::CustomClassHolder {
+    Kind in[NIN];
+    bool need[NIN];
+    bool normalize, reverse, last;
+  };
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& A, const MaybeTensor& in_gate_,
+                               const MaybeTensor& h0_, const MaybeTensor& seq_, bool normalize, bool reverse, bool want_last) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor in_gate = opt(in_gate_), h0 = opt(h0_), seq = opt(seq_);
+    const GatedScan s = GatedScan::make(x, gate, A, in_gate, h0, seq, normalize, reverse);
+    GatedScan::Out o = s.forward(want_last, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({s.x, s.gate, s.A, s.in_gate, s.h0, s.seq, o.saved});   // (the inputs themselves where the kernels read those)
+    auto r = c10::make_intrusive<Record>();
+    const Tensor* in[NIN] = {&x, &gate, &A, &in_gate, &h0};
+    for (int i = 0; i < NIN; ++i) {
+      r->in[i] = Kind(*in[i]);
+      r->need[i] = in[i]->defined() && in[i]->requires_grad();
+    }
+    r->normalize = normalize;
+    r->reverse = reverse;
+    r->last = want_last;
+    keep(ctx, std::move(r));
+    variable_list out{cast(o.y, x.scalar_type())};
+    if (want_last) out.push_back(o.last);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    first_derivatives_only("gated_scan");
+    const variable_list v = ctx->get_saved_variables();
+    const auto in = kept<Record>(ctx);
+    GatedScan s;
+    s.x = v[0];
+    s.gate = v[1];
+    s.A = v[2];
+    s.in_gate = v[3];
+    s.h0 = v[4];
+    s.seq = v[5];
+    s.normalize = in->normalize;
+    s.reverse = in->reverse;
+    const c10::DeviceGuard guard(s.x.device());
+    const Tensor dy = kernel_operand(grads[0], s.x.scalar_type()), dlast = in->last && grads[1].defined() ? f32c(grads[1].resolve_neg()) : Tensor();
+    variable_list out(NIN + 4);
+    if (!dy.defined() && !dlast.defined()) return out;
+    Tensor g[NIN];
+    for (int i = 0; i < NIN; ++i)
+      if (in->need[i]) g[i] = fresh(in->in[i].sizes, s.x, i == 2 || i == 4 ? at::kFloat : s.x.scalar_type());
+    if (s.empty()) {
+      if (g[2].defined()) g[2].zero_();
+      if (g[4].defined()) dlast.defined() ? g[4].copy_(dlast) : g[4].zero_();
+    } else {
+      issm_gated_scan_args a = s.args();
+      a.saved = data(v[6]);
+      if (dy.defined()) {
+        a.dy = data(dy);
+        a.dy_stride[0] = dy.stride(0);
+        a.dy_stride[1] = dy.stride(1);
+      }
+      a.dlast = data<const float>(dlast);
+      a.dx = data(g[0]);
+      a.dgate = data(g[1]);
+      a.dA = data<float>(g[2]);
+      a.din_gate = data(g[3]);
+      a.dh0 = data<float>(g[4]);
+      const Tensor ws = s.workspace(a, true);
+      check(issm_gated_scan_bwd(&a), "issm_gated_scan_bwd");
+    }
+    for (int i = 0; i < NIN; ++i)
+      if (g[i].defined()) out[i] = cast(g[i], in->in[i].type);
+    return out;
+  }
+};
+
+void require_shape(bool ok, const std::string& name, const char* want, const Tensor& t) {
+  if (!ok) raise_py(PyExc_ValueError, name + " must be " + want + ", got " + shape_text(t));
+}
+void require_type(bool ok, const std::string& name, const char* want, const Tensor& t) {
+  if (!ok) raise_py(PyExc_TypeError, name + " must be " + want + ", got " + toString(t.scalar_type()));
+}
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+
+std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Tensor& A, const MaybeTensor& in_gate_, const MaybeTensor& h0_,
+                               const MaybeTensor& seq_, bool normalize, bool reverse, bool want_last) {
+  const Tensor in_gate = opt(in_gate_), h0 = opt(h0_), seq = opt(seq_);
+  require_gpu(x, "x");
+  require_beside(x, {&gate, &A, &in_gate, &h0, &seq});
+  require_shape(x.dim() == 3, "x", "(batch, seqlen, channels)", x);
+  require_type(at::isFloatingType(x.scalar_type()), "x", "of a floating type", x);
+  for (const Tensor* t : {&gate, &in_gate})
+    if (t->defined()) {
+      require_shape(t->sizes() == x.sizes(), t == &gate ? "gate" : "in_gate", "of x's shape", *t);
+      require_type(at::isFloatingType(t->scalar_type()), t == &gate ? "gate" : "in_gate", "of a floating type", *t);
+    }
+  require_shape(A.dim() == 1 && A.size(0) == x.size(2), "A", "(channels,)", A);
+  require_type(at::isFloatingType(A.scalar_type()), "A", "of a floating type", A);
+  if (h0.defined()) {
+    require_shape(h0.sizes() == at::IntArrayRef({x.size(0), x.size(2)}), "initial_states", "(batch, channels)", h0);
+    require_type(at::isFloatingType(h0.scalar_type()), "initial_states", "of a floating type", h0);
+  }
+  if (seq.defined()) {
+    require_shape(seq.sizes() == at::IntArrayRef({x.size(0), x.size(1)}), "seq_idx", "(batch, seqlen)", seq);
+    require_type(at::isIntegralType(seq.scalar_type(), false), "seq_idx", "of an integer type", seq);
+  }
+  for (int i = 0; i < 3; ++i) require_shape(x.size(i) <= INT32_MAX, "x", "of fewer than 2^31 entries a dimension", x);
+  py::gil_scoped_release release;
+  if (recorded({&x, &gate, &A, &in_gate, &h0})) return GatedScanFn::apply(x, gate, A, in_gate_, h0_, seq_, normalize, reverse, want_last);
+  const c10::DeviceGuard guard(x.device());
+  GatedScan::Out o = GatedScan::make(x, gate, A, in_gate, h0, seq, normalize, reverse).forward(want_last, false);
+  std::vector<Tensor> out{cast(o.y, x.scalar_type())};
+  if (want_last) out.push_back(o.last);
+  return out;
+}
+
+Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, const Tensor& state, const MaybeTensor& in_gate_,
+                       const MaybeTensor& at_, bool normalize) {
+  const Tensor in_gate = opt(in_gate_), at = opt(at_);
+  require_gpu(x, "x");
+  require_beside(x, {&gate, &A, &state, &in_gate, &at});
+  require_shape(x.dim() == 2, "x", "(rows, channels)", x);
+  require_type(at::isFloatingType(x.scalar_type()), "x", "of a floating type", x);
+  for (const Tensor* t : {&gate, &in_gate})
+    if (t->defined()) {
+      require_shape(t->sizes() == x.sizes(), t == &gate ? "gate" : "in_gate", "of x's shape", *t);
+      require_type(at::isFloatingType(t->scalar_type()), t == &gate ? "gate" : "in_gate", "of a floating type", *t);
+    }
+  require_shape(A.dim() == 1 && A.size(0) == x.size(1), "A", "(channels,)", A);
+  require_type(at::isFloatingType(A.scalar_type()), "A", "of a floating type", A);
+  require_shape(state.dim() == 2 && state.size(1) == x.size(1), "state", "(slots, channels)", state);
+  require_type(state.scalar_type() == at::kFloat, "state", "float32 (it is updated in place)", state);
+  const int64_t rows = x.size(0), C = x.size(1), slots = state.size(0);
+  require((C <= 1 || state.stride(1) == 1) && (slots <= 1 || state.stride(0) >= C) && !state.is_neg(),
+          "state must have contiguous channels and slots that do not overlap (it is updated in place)");
+  if (at.defined()) {
+    require_shape(at.dim() == 1 && at.size(0) == rows, "state_indices", "(rows,)", at);
+    require_type(is_index(at), "state_indices", "int32 or int64", at);
+  } else {
+    require_shape(slots == rows, "state", "(rows, channels) without state_indices", state);
+  }
+  require_shape(rows <= INT32_MAX && C <= INT32_MAX, "x", "of fewer than 2^31 entries a dimension", x);
+  if (recorded({&x, &gate, &A, &state, &in_gate}))
+    raise_py(PyExc_RuntimeError, "gated_scan_step has no backward: call it under torch.no_grad(), or gated_scan");
+  py::gil_scoped_release release;
+  const c10::DeviceGuard guard(x.device());
+  const at::ScalarType io = kernel_type(x.scalar_type());
+  const Tensor xk = kernel_operand(x, io), gk = kernel_operand(gate, io), ik = kernel_operand(in_gate, io), Ak = f32c(A.resolve_neg()),
+               ak = at.defined() ? at.contiguous() : at;
+  const Tensor y = fresh(x.sizes(), x, io);
+  if (x.numel() == 0) return cast(y, x.scalar_type());
+  if (slots == 0) return cast(y.zero_(), x.scalar_type());
+  issm_gated_scan_step_args a{};
+  a.rows = (int32_t)rows;
+  a.channels = (int32_t)C;
+  a.slots = slots;
+  a.dtype = code(io);
+  a.flags = normalize ? ISSM_GS_NORMALIZE : 0u;
+  a.x = data(xk);
+  a.gate = data(gk);
+  a.in_gate = data(ik);
+  a.x_stride = xk.stride(0);
+  a.gate_stride = gk.stride(0);
+  a.in_gate_stride = ik.defined() ? ik.stride(0) : 0;
+  a.A = data<const float>(Ak);
+  a.state = data<float>(state);
+  a.state_stride = state.stride(0);
+  a.slots_of = data(ak);
+  a.slots_64 = ak.defined() && ak.scalar_type() == at::kLong;
+  a.y = data(y);
+  a.stream = stream_of(x);
+  check(issm_gated_scan_step(&a), "issm_gated_scan_step");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();   // (what saved it for a backward is told)
+  return cast(y, x.scalar_type());
+}
+
+// ----------------------------------------------------------------------------------------------------- rotary positions
+struct Rotary {
+  Tensor x[2], w[2], table, pos;   // as the kernels read them; w undefined: no norm
+  bool inter = false;
+  double eps = 0;
+
+  static Rotary make(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& table, const Tensor& pos, double eps,
+                     bool inter) {
+    Rotary r;
+    const at::ScalarType io = kernel_type(q.scalar_type());
+    r.x[0] = kernel_operand(q, io);
+    r.x[1] = kernel_operand(k, io);
+    if (wq.defined()) {
+      const at::ScalarType wt = is_kernel_type(wq.scalar_type()) && (!wk.defined() || wk.scalar_type() == wq.scalar_type()) ? wq.scalar_type() : at::kFloat;
+      r.w[0] = kernel_operand(wq, wt);
+      r.w[1] = kernel_operand(wk, wt);
+    }
+    r.table = f32c(table.resolve_neg());
+    r.pos = pos;
+    r.eps = eps;
+    r.inter = inter;
+    return r;
+  }
+  const Tensor& any() const { return x[0].defined() ? x[0] : x[1]; }
+  // sizes: of the queries and keys, whether or not they are here; has: the sides of this call
+  issm_rotary_args args(const at::DimVector (&sizes)[2], const bool (&has)[2], const Tensor& like) const {
+    issm_rotary_args a{};
+    a.batch = (int32_t)sizes[0][0];
+    a.seqlen = (int32_t)sizes[0][1];
+    a.headdim = (int32_t)sizes[0][3];
+    a.rot = (int32_t)table.size(1);
+    a.dtype = code(like.scalar_type());
+    a.flags = inter ? ISSM_ROT_INTERLEAVED : 0u;
+    a.eps = (float)eps;
+    for (int i = 0; i < 2; ++i) {
+      if (!has[i]) continue;
+      a.heads[i] = (int32_t)sizes[i][2];
+      a.w[i] = data(w[i]);
+      if (w[i].defined()) a.weight_dtype = code(w[i].scalar_type());
+    }
+    a.table = data<const float>(table);
+    a.table_rows = table.size(0);
+    if (pos.defined()) {
+      a.positions = data(pos);
+      a.positions_stride[0] = pos.dim() == 2 ? pos.stride(0) : 0;
+      a.positions_stride[1] = pos.stride(-1);
+      a.positions_64 = pos.scalar_type() == at::kLong;
+    }
+    a.stream = stream_of(like);
+    return a;
+  }
+  static void strided(const Tensor& t, const void*& p, int64_t (&stride)[3]) {
+    p = data(t);
+    for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+  }
+  // x's sides turned (back: the other way) by the norm's or the plain entry point; undefined ones stay so
+  std::array<Tensor, 2> turn(const at::DimVector (&sizes)[2], bool back) const {
+    const bool has[2] = {x[0].defined() && x[0].numel() > 0, x[1].defined() && x[1].numel() > 0};
+    std::array<Tensor, 2> y;
+    for (int i = 0; i < 2; ++i)
+      if (x[i].defined()) y[i] = fresh(x[i].sizes(), x[i], x[i].scalar_type());
+    if (!has[0] && !has[1]) return y;
+    issm_rotary_args a = args(sizes, has, any());
+    if (back) a.flags |= ISSM_ROT_BACK;
+    for (int i = 0; i < 2; ++i)
+      if (has[i]) {
+        strided(x[i], a.x[i], a.x_stride[i]);
+        a.y[i] = data(y[i]);
+      }
+    if (w[0].defined()) check(issm_rotary_norm_fwd(&a), "issm_rotary_norm_fwd");
+    else check(issm_rotary(&a), "issm_rotary");
+    return y;
+  }
+};
+
+// Inputs 0 .. 3 of the node: q, k, q_weight, k_weight (the weights absent: the rotation alone)
+struct RotaryFn : public Function<RotaryFn> {
+  struct Record : torch::CustomClassHolder {
+    Kind in[4];
+    bool need[4];
+    bool inter, norm;
+    double eps;
+    at::ScalarType io;
+  };
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const MaybeTensor& k_, const MaybeTensor& wq_, const MaybeTensor& wk_,
+                               const Tensor& table, const MaybeTensor& pos_, double eps, bool inter) {
+    const c10::DeviceGuard guard(q.device());
+    const Tensor k = opt(k_), wq = opt(wq_), wk = opt(wk_), pos = opt(pos_);
+    const Rotary s = Rotary::make(q, k, wq, wk, table, pos, eps, inter);
+    auto r = c10::make_intrusive<Record>();
+    const Tensor* in[4] = {&q, &k, &wq, &wk};
+    for (int i = 0; i < 4; ++i) {
+      r->in[i] = Kind(*in[i]);
+      r->need[i] = in[i]->defined() && in[i]->requires_grad();
+    }
+    r->inter = inter;
+    r->norm = wq.defined();
+    r->eps = eps;
+    r->io = s.x[0].scalar_type();
+    const auto y = s.turn({r->in[0].sizes, r->in[1].sizes}, false);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward(r->norm ? variable_list{s.table, s.pos, s.x[0], s.x[1], s.w[0], s.w[1]} : variable_list{s.table, s.pos});
+    keep(ctx, std::move(r));
+    variable_list out{cast(y[0], q.scalar_type())};
+    if (k.defined()) out.push_back(cast(y[1], k.scalar_type()));
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto in = kept<Record>(ctx);
+    first_derivatives_only(in->norm ? "qk_norm_rotary" : "rotary");
+    const variable_list v = ctx->get_saved_variables();
+    variable_list out(8);
+    Rotary s;
+    s.table = v[0];
+    s.pos = v[1];
+    s.inter = in->inter;
+    s.eps = in->eps;
+    const c10::DeviceGuard guard(s.table.device());
+    Tensor dy[2];
+    bool has[2];
+    for (int i = 0; i < 2; ++i) {
+      const bool wanted = in->need[i] || in->need[2 + i];
+      if (wanted && (size_t)i < grads.size() && grads[i].defined()) dy[i] = kernel_operand(grads[i], in->io);
+      has[i] = dy[i].defined() && dy[i].numel() > 0;
+    }
+    const at::DimVector sizes[2] = {in->in[0].sizes, in->in[1].sizes};
+    if (!in->norm) {
+      s.x[0] = dy[0];
+      s.x[1] = dy[1];
+      const auto dx = s.turn(sizes, true);
+      for (int i = 0; i < 2; ++i)
+        if (dx[i].defined()) out[i] = cast(dx[i], in->in[i].type);
+      return out;
+    }
+    Tensor dx[2], dw[2], scratch;
+    for (int i = 0; i < 2; ++i) {
+      s.x[i] = v[2 + i];
+      s.w[i] = v[4 + i];
+      if (!dy[i].defined()) continue;
+      dx[i] = fresh(sizes[i], dy[i], in->io);
+      if (in->need[2 + i]) dw[i] = has[i] ? fresh({sizes[i][3]}, dy[i], s.w[i].scalar_type()) : at::zeros({sizes[i][3]}, s.w[i].options());
+    }
+    if (has[0] || has[1]) {
+      issm_rotary_args a = s.args(sizes, has, has[0] ? dy[0] : dy[1]);
+      for (int i = 0; i < 2; ++i)
+        if (has[i]) {
+          Rotary::strided(s.x[i], a.x[i], a.x_stride[i]);
+          Rotary::strided(dy[i], a.dy[i], a.dy_stride[i]);
+          a.dx[i] = data(dx[i]);
+          a.dw[i] = data(dw[i]);
+        }
+      size_t n = 0;
+      check(issm_rotary_norm_bwd_bytes(&a, &n), "issm_rotary_norm_bwd_bytes");
+      scratch = fresh({(int64_t)n}, dx[has[0] ? 0 : 1], at::kByte);
+      a.scratch = data(scratch);
+      a.scratch_bytes = n;
+      check(issm_rotary_norm_bwd(&a), "issm_rotary_norm_bwd");
+    }
+    for (int i = 0; i < 2; ++i) {
+      if (dx[i].defined() && in->need[i]) out[i] = cast(dx[i], in->in[i].type);
+      if (dw[i].defined()) out[2 + i] = cast(dw[i], in->in[2 + i].type);
+    }
+    return out;
+  }
+};
+
+std::vector<Tensor> rotary(const Tensor& q, const MaybeTensor& k_, const MaybeTensor& wq_, const MaybeTensor& wk_, const Tensor& table,
+                           const MaybeTensor& pos_, double eps, bool inter) {
+  const Tensor k = opt(k_), wq = opt(wq_), wk = opt(wk_), pos = opt(pos_);
+  require_gpu(q, "q");
+  require_beside(q, {&k, &wq, &wk, &table, &pos});
+  require_shape(q.dim() == 4, "q", "(batch, seqlen, heads, headdim)", q);
+  require_type(at::isFloatingType(q.scalar_type()), "q", "of a floating type", q);
+  const int64_t B = q.size(0), L = q.size(1), D = q.size(3);
+  if (k.defined()) {
+    require_shape(k.dim() == 4 && k.size(0) == B && k.size(1) == L && k.size(3) == D, "k", "(batch, seqlen, kv_heads, headdim) beside q", k);
+    require_type(at::isFloatingType(k.scalar_type()), "k", "of a floating type", k);
+  }
+  for (const Tensor* w : {&wq, &wk})
+    if (w->defined()) {
+      require_shape(w->dim() == 1 && w->size(0) == D, w == &wq ? "q_weight" : "k_weight", "(headdim,)", *w);
+      require_type(at::isFloatingType(w->scalar_type()), w == &wq ? "q_weight" : "k_weight", "of a floating type", *w);
+    }
+  require_shape(table.dim() == 2 && table.size(1) >= 2 && table.size(1) % 2 == 0 && table.size(1) <= D && table.size(0) >= 1, "table",
+                "(positions, turned features) with an even number of at most headdim features", table);
+  require_type(at::isFloatingType(table.scalar_type()), "table", "of a floating type", table);
+  require(!(at::GradMode::is_enabled() && table.requires_grad()), "table has no gradient: detach it");
+  if (pos.defined()) {
+    require_shape((pos.dim() == 2 && pos.size(0) == B && pos.size(1) == L) || (pos.dim() == 1 && pos.size(0) == L), "positions",
+                  "(batch, seqlen) or (seqlen,)", pos);
+    require_type(is_index(pos), "positions", "int32 or int64", pos);
+  } else {
+    require_shape(table.size(0) >= L, "table", "of as many rows as there are tokens, without positions", table);
+  }
+  for (int i = 0; i < 4; ++i)
+    require_shape(q.size(i) <= INT32_MAX && (!k.defined() || k.size(i) <= INT32_MAX), "q", "of fewer than 2^31 entries a dimension", q);
+  py::gil_scoped_release release;
+  if (recorded({&q, &k, &wq, &wk})) return RotaryFn::apply(q, k_, wq_, wk_, table, pos_, eps, inter);
+  const c10::DeviceGuard guard(q.device());
+  const auto y = Rotary::make(q, k, wq, wk, table, pos, eps, inter).turn({at::DimVector(q.sizes()), at::DimVector(k.defined() ? k.sizes() : q.sizes())}, false);
+  std::vector<Tensor> out{cast(y[0], q.scalar_type())};
+  if (k.defined()) out.push_back(cast(y[1], k.scalar_type()));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1340,4 +1821,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("runs_twice", &runs_twice);
   m.def("scan_core", &scan_core);
   m.def("scan_layer", &scan_layer);
+  m.def("gated_scan", &gated_scan);
+  m.def("gated_scan_step", &gated_scan_step);
+  m.def("rotary", &rotary);
 }

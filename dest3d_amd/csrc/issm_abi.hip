@@ -11,6 +11,7 @@
 
 #include "../../include/issm.h"
 #include "issm_dev.h"
+#include "rotary_dev.h"
 
 namespace issm {
 int launch_chunk_local(const KP& p, float* states, float* cs_last, float* cabt, bool any, hipStream_t st);
@@ -87,6 +88,10 @@ int launch_dwconv_bwd(const DwConvP& p, hipStream_t st);
 int pgen_bwd_blocks(long tokens);
 int launch_pgen_fwd(const PGenP& p, hipStream_t st);
 int launch_pgen_bwd(const PGenP& p, hipStream_t st);
+int launch_gscan(GScanP p, bool bf, bool nrm, bool back, hipStream_t st);
+int launch_gscan_step(GStepP p, bool bf, bool nrm, hipStream_t st);
+int launch_rotary(RotP p, bool bf, bool inter, bool norm, hipStream_t st);
+int launch_rotary_norm_bwd(RotP p, bool bf, bool inter, hipStream_t st);
 }  // namespace issm
 
 using namespace issm;
@@ -1420,6 +1425,214 @@ int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t 
   PN2_PTRS("three_interpolate_grad_cl", grad_out, idx, weight, grad_points_cl);
   return launched(launch_scatter_channel_last(true, b, c, m, n, grad_out, idx, weight, grad_points_cl, (hipStream_t)stream),
                   "three_interpolate_grad_cl");
+}
+
+// ---- gated linear recurrence --------------------------------------------------------------------
+static int gscan_sizes(const issm_gated_scan_args* a) {
+  if (!a) return fail(ISSM_E_NULL, "gated_scan: args is NULL");
+  if (a->batch < 1 || a->seqlen < 1 || a->channels < 1 || a->seqlen > (1 << 30))
+    return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d", a->batch, a->seqlen, a->channels);
+  if ((int64_t)a->batch * gscan_blocks(a->channels) * gscan_tiles(a->seqlen) >= (1 << 22))
+    return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d are too many tiles", a->batch, a->seqlen, a->channels);
+  if (a->dtype != ISSM_F32 && a->dtype != ISSM_BF16) return fail(ISSM_E_DTYPE, "gated_scan: dtype %d", a->dtype);
+  if (a->flags & ~(ISSM_GS_NORMALIZE | ISSM_GS_REVERSE)) return fail(ISSM_E_UNSUPPORTED, "gated_scan: flags 0x%x", a->flags);
+  return ISSM_OK;
+}
+
+int issm_gated_scan_saved_bytes(const issm_gated_scan_args* a, size_t* out) {
+  int rc = gscan_sizes(a);
+  if (rc) return rc;
+  if (!out) return fail(ISSM_E_NULL, "out is NULL");
+  *out = (size_t)a->batch * gscan_tiles(a->seqlen) * a->channels * sizeof(float);
+  return ISSM_OK;
+}
+
+int issm_gated_scan_workspace_bytes(const issm_gated_scan_args* a, int32_t backward, size_t* out) {
+  int rc = gscan_sizes(a);
+  if (rc) return rc;
+  if (!out) return fail(ISSM_E_NULL, "out is NULL");
+  *out = backward ? (size_t)a->batch * a->channels * sizeof(float) : 0;
+  return ISSM_OK;
+}
+
+static int gscan_call(const issm_gated_scan_args* a, bool back) {
+  size_t need = 0;
+  int rc = issm_gated_scan_workspace_bytes(a, back, &need);
+  if (rc) return rc;
+  if (!a->x || !a->gate || !a->A) return fail(ISSM_E_NULL, "gated_scan: x/gate/A is NULL");
+  if (!back && !a->y) return fail(ISSM_E_NULL, "gated_scan: y is NULL");
+  if (back && !a->saved) return fail(ISSM_E_NULL, "gated_scan bwd: saved is NULL");
+  if (back && a->din_gate && !a->in_gate) return fail(ISSM_E_NULL, "gated_scan bwd: din_gate without in_gate");
+  GScanP p{};
+  p.B = a->batch;
+  p.L = a->seqlen;
+  p.C = a->channels;
+  const bool bf = a->dtype == ISSM_BF16, reverse = a->flags & ISSM_GS_REVERSE;
+  const int64_t size = bf ? 2 : 4, end = a->seqlen - 1;
+  const int64_t* strides[5] = {a->x_stride, a->gate_stride, a->in_gate_stride, a->dy_stride, a->seq_idx_stride};
+  const void* in[5] = {a->x, a->gate, a->in_gate, back ? a->dy : nullptr, a->seq_idx};
+  const void** to[4] = {&p.x, &p.g, &p.i, &p.dy};
+  long* batch[4] = {&p.xb, &p.gb, &p.ib, &p.dyb};
+  long* token[4] = {&p.xl, &p.gl, &p.il, &p.dyl};
+  for (int i = 0; i < 5; ++i) {
+    if (!in[i]) continue;
+    if (strides[i][0] < 0 || strides[i][1] < 0)
+      return fail(ISSM_E_STRIDE, "gated_scan: negative strides (%lld, %lld)", (long long)strides[i][0], (long long)strides[i][1]);
+    if (i == 4) break;
+    *to[i] = (const char*)in[i] + (reverse ? end * strides[i][1] * size : 0);
+    *batch[i] = strides[i][0];
+    *token[i] = reverse ? -strides[i][1] : strides[i][1];
+  }
+  if (a->seq_idx) {
+    p.ids = a->seq_idx + (reverse ? end * a->seq_idx_stride[1] : 0);
+    p.ids_b = a->seq_idx_stride[0];
+    p.ids_l = reverse ? -a->seq_idx_stride[1] : a->seq_idx_stride[1];
+  }
+  p.yb = (long)a->seqlen * a->channels;
+  p.yl = reverse ? -(long)a->channels : a->channels;
+  auto first = [&](void* t) { return t && reverse ? (void*)((char*)t + end * a->channels * size) : t; };
+  p.A = a->A;
+  p.h0 = a->h0;
+  p.hs = (float*)a->saved;
+  if (back) {
+    p.dx = first(a->dx);
+    p.dg = first(a->dgate);
+    p.di = first(a->din_gate);
+    p.dlast = a->dlast;
+    p.dh0 = a->dh0;
+    p.dA = a->dA;
+    if (need && (!a->workspace || a->workspace_bytes < need))
+      return fail(ISSM_E_WORKSPACE, "gated_scan bwd: %zu bytes of workspace, %zu needed", a->workspace_bytes, need);
+    p.part = a->dA ? (float*)a->workspace : nullptr;
+  } else {
+    p.y = first(a->y);
+    p.last = a->last;
+  }
+  return launched(launch_gscan(p, bf, a->flags & ISSM_GS_NORMALIZE, back, (hipStream_t)a->stream), back ? "gated_scan_bwd" : "gated_scan_fwd");
+}
+
+int issm_gated_scan_fwd(const issm_gated_scan_args* a) { return gscan_call(a, false); }
+int issm_gated_scan_bwd(const issm_gated_scan_args* a) { return gscan_call(a, true); }
+
+int issm_gated_scan_step(const issm_gated_scan_step_args* a) {
+  if (!a) return fail(ISSM_E_NULL, "gated_scan_step: args is NULL");
+  if (a->rows < 1 || a->channels < 1 || a->slots < 1 || (int64_t)a->rows * ((a->channels + 1023) / 1024) >= (1 << 23))
+    return fail(ISSM_E_SHAPE, "gated_scan_step: rows=%d channels=%d slots=%lld", a->rows, a->channels, (long long)a->slots);
+  if (a->dtype != ISSM_F32 && a->dtype != ISSM_BF16) return fail(ISSM_E_DTYPE, "gated_scan_step: dtype %d", a->dtype);
+  if (a->flags & ~ISSM_GS_NORMALIZE) return fail(ISSM_E_UNSUPPORTED, "gated_scan_step: flags 0x%x", a->flags);
+  if (!a->x || !a->gate || !a->A || !a->state || !a->y) return fail(ISSM_E_NULL, "gated_scan_step: x/gate/A/state/y is NULL");
+  if (!a->slots_of && a->slots < a->rows)
+    return fail(ISSM_E_SHAPE, "gated_scan_step: %d rows, %lld states", a->rows, (long long)a->slots);
+  if (a->x_stride < 0 || a->gate_stride < 0 || a->in_gate_stride < 0 || (a->slots > 1 && a->state_stride < a->channels))
+    return fail(ISSM_E_STRIDE, "gated_scan_step: strides");
+  GStepP p{};
+  p.rows = a->rows;
+  p.C = a->channels;
+  p.slots = a->slots;
+  p.state_s = a->state_stride;
+  p.x = a->x;
+  p.g = a->gate;
+  p.i = a->in_gate;
+  p.xs = a->x_stride;
+  p.gs = a->gate_stride;
+  p.is = a->in_gate_stride;
+  p.A = a->A;
+  p.state = a->state;
+  p.at = a->slots_of;
+  p.at64 = a->slots_64;
+  p.y = a->y;
+  return launched(launch_gscan_step(p, a->dtype == ISSM_BF16, a->flags & ISSM_GS_NORMALIZE, (hipStream_t)a->stream), "gated_scan_step");
+}
+
+// ---- rotary positions -----------------------------------------------------------------------------
+static int rotary_sizes(const issm_rotary_args* a) {
+  if (!a) return fail(ISSM_E_NULL, "rotary: args is NULL");
+  if (a->batch < 1 || a->seqlen < 1 || a->headdim < 1 || a->heads[0] < 0 || a->heads[1] < 0 || a->heads[0] + a->heads[1] < 1)
+    return fail(ISSM_E_SHAPE, "rotary: batch=%d seqlen=%d heads=%d, %d headdim=%d", a->batch, a->seqlen, a->heads[0], a->heads[1], a->headdim);
+  if (a->rot < 2 || a->rot % 2 || a->rot > a->headdim) return fail(ISSM_E_SHAPE, "rotary: %d of %d features turned", a->rot, a->headdim);
+  if (a->headdim > ROT_MAX_D) return fail(ISSM_E_UNSUPPORTED, "rotary: headdim %d > %d", a->headdim, ROT_MAX_D);
+  if ((int64_t)a->heads[0] + a->heads[1] > (1 << 20) || (int64_t)a->batch * a->seqlen >= (1LL << 31) ||
+      (int64_t)a->batch * a->seqlen * (a->heads[0] + a->heads[1]) >= (1LL << 31))
+    return fail(ISSM_E_SHAPE, "rotary: 2^31 rows or more");
+  if ((unsigned)a->dtype > 1u || (unsigned)a->weight_dtype > 1u) return fail(ISSM_E_DTYPE, "rotary: unknown dtype");
+  if (a->flags & ~(ISSM_ROT_INTERLEAVED | ISSM_ROT_BACK)) return fail(ISSM_E_UNSUPPORTED, "rotary: flags 0x%x", a->flags);
+  return ISSM_OK;
+}
+
+static int rotary_params(const issm_rotary_args* a, RotP* p, bool norm, bool back) {
+  int rc = rotary_sizes(a);
+  if (rc) return rc;
+  *p = RotP{};
+  p->L = a->seqlen;
+  p->D = a->headdim;
+  p->R = a->rot;
+  p->tokens = a->batch * a->seqlen;
+  for (int i = 0; i < 2; ++i) {
+    if (!a->heads[i]) continue;
+    p->H[i] = a->heads[i];
+    p->x[i] = a->x[i];
+    p->y[i] = back ? a->dx[i] : a->y[i];
+    if (!p->x[i] || !p->y[i]) return fail(ISSM_E_NULL, "rotary: x/y/dx is NULL");
+    if (norm && !(p->w[i] = a->w[i])) return fail(ISSM_E_NULL, "rotary: w is NULL");
+    if (back && !(p->dy[i] = a->dy[i])) return fail(ISSM_E_NULL, "rotary bwd: dy is NULL");
+    for (int j = 0; j < 3; ++j) {
+      p->s[i][j] = a->x_stride[i][j];
+      p->ds[i][j] = back ? a->dy_stride[i][j] : 0;
+      if (p->s[i][j] < 0 || p->ds[i][j] < 0) return fail(ISSM_E_STRIDE, "rotary: negative stride");
+    }
+    p->dw[i] = back ? a->dw[i] : nullptr;
+  }
+  if (!a->table) return fail(ISSM_E_NULL, "rotary: table is NULL");
+  if (a->table_rows < 1 || (!a->positions && a->table_rows < a->seqlen))
+    return fail(ISSM_E_SHAPE, "rotary: %d tokens, %lld rows of the table", a->seqlen, (long long)a->table_rows);
+  if (a->positions && (a->positions_stride[0] < 0 || a->positions_stride[1] < 0)) return fail(ISSM_E_STRIDE, "rotary: negative stride");
+  p->table = a->table;
+  p->rows = a->table_rows;
+  p->pos = a->positions;
+  p->pos_b = a->positions_stride[0];
+  p->pos_l = a->positions_stride[1];
+  p->pos64 = a->positions_64;
+  p->w_bf = a->weight_dtype == ISSM_BF16;
+  p->eps = a->eps;
+  p->sign = a->flags & ISSM_ROT_BACK ? -1.0f : 1.0f;
+  return ISSM_OK;
+}
+
+int issm_rotary(const issm_rotary_args* a) {
+  RotP p;
+  int rc = rotary_params(a, &p, false, false);
+  if (rc) return rc;
+  return launched(launch_rotary(p, a->dtype == ISSM_BF16, a->flags & ISSM_ROT_INTERLEAVED, false, (hipStream_t)a->stream), "rotary");
+}
+
+int issm_rotary_norm_fwd(const issm_rotary_args* a) {
+  RotP p;
+  int rc = rotary_params(a, &p, true, false);
+  if (rc) return rc;
+  if (a->flags & ISSM_ROT_BACK) return fail(ISSM_E_UNSUPPORTED, "rotary_norm_fwd: flags 0x%x", a->flags);
+  return launched(launch_rotary(p, a->dtype == ISSM_BF16, a->flags & ISSM_ROT_INTERLEAVED, true, (hipStream_t)a->stream), "rotary_norm_fwd");
+}
+
+int issm_rotary_norm_bwd_bytes(const issm_rotary_args* a, size_t* out) {
+  int rc = rotary_sizes(a);
+  if (rc) return rc;
+  if (!out) return fail(ISSM_E_NULL, "out is NULL");
+  const int64_t tokens = (int64_t)a->batch * a->seqlen;
+  *out = (size_t)(rotary_bwd_blocks(tokens * a->heads[0]) + rotary_bwd_blocks(tokens * a->heads[1])) * a->headdim * sizeof(float);
+  return ISSM_OK;
+}
+
+int issm_rotary_norm_bwd(const issm_rotary_args* a) {
+  RotP p;
+  int rc = rotary_params(a, &p, true, true);
+  if (rc) return rc;
+  if (a->flags & ISSM_ROT_BACK) return fail(ISSM_E_UNSUPPORTED, "rotary_norm_bwd: flags 0x%x", a->flags);
+  size_t need = 0;
+  issm_rotary_norm_bwd_bytes(a, &need);
+  if (!a->scratch || a->scratch_bytes < need)
+    return fail(ISSM_E_WORKSPACE, "rotary_norm_bwd: %zu bytes of scratch, %zu needed", a->scratch_bytes, need);
+  p.part = (float*)a->scratch;
+  return launched(launch_rotary_norm_bwd(p, a->dtype == ISSM_BF16, a->flags & ISSM_ROT_INTERLEAVED, (hipStream_t)a->stream), "rotary_norm_bwd");
 }
 
 }  // extern "C"

@@ -726,6 +726,118 @@ int issm_pn2_group_points_grad_cl(int32_t b, int32_t c, int32_t n, int32_t npoin
 int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t m, const float* grad_out,
                                        const int32_t* idx, const float* weight, float* grad_points_cl, void* stream);
 
+/* ---- gated linear recurrence -----------------------------------------------------------------
+ * A state of one number for each channel, decayed by a gate and fed by the input:
+ *   r = sigmoid(gate), l = A r, a = exp(l), beta = sqrt(1 - a^2) (ISSM_GS_NORMALIZE; else 1), u = sigmoid(in_gate) x (x without in_gate)
+ *   h_t = a_t h_{t-1} + beta_t u_t,   y = h,   last = the state behind the last token
+ * A <= 0 with ISSM_GS_NORMALIZE (a positive entry gives NaN there).  x, gate, in_gate, dy (B, L, C) in `dtype`, channels contiguous, element
+ * strides of batch and token (0 repeats); y, dx, dgate, din_gate (B, L, C) contiguous in `dtype`; A, dA (C), h0, last, dlast, dh0 (B, C) fp32
+ * contiguous.  seq_idx (B, L) int32 or NULL: every change of id from a token to the next cuts the recurrence, and no value passes, whatever it
+ * is; h0 counts as id 0: it feeds a row whose first token has id 0 and no other.  ISSM_GS_REVERSE walks from the last token to the first ("first"
+ * and "last" above in the walk's order).  States, decays and sums are fp32; results are bit-reproducible.
+ * saved: issm_gated_scan_saved_bytes, the states that the backward starts its tiles from; NULL in a forward that none follows.  workspace:
+ * issm_gated_scan_workspace_bytes (may be 0).  Backward: dy, dlast NULL = zero, dx, dgate, din_gate, dA, dh0 NULL = not wanted; where beta = 0 (nothing
+ * decays) it has no derivative: its part of dgate and dA is taken as 0. */
+#define ISSM_GS_NORMALIZE 1u
+#define ISSM_GS_REVERSE 2u
+typedef struct issm_gated_scan_args {
+  int32_t batch, seqlen, channels;
+  int32_t dtype;
+  uint32_t flags;
+  const void* x;
+  const void* gate;
+  const void* in_gate; /* optional */
+  int64_t x_stride[2], gate_stride[2], in_gate_stride[2];
+  const float* A;
+  const float* h0;        /* optional */
+  const int32_t* seq_idx; /* optional */
+  int64_t seq_idx_stride[2];
+  void* y;
+  float* last; /* optional */
+  void* saved;
+  /* backward */
+  const void* dy;
+  int64_t dy_stride[2];
+  const float* dlast;
+  void* dx;
+  void* dgate;
+  void* din_gate;
+  float* dA;
+  float* dh0;
+  void* workspace; /* 256-byte aligned */
+  size_t workspace_bytes;
+  void* stream;
+} issm_gated_scan_args;
+
+int issm_gated_scan_saved_bytes(const issm_gated_scan_args* args, size_t* out);
+int issm_gated_scan_workspace_bytes(const issm_gated_scan_args* args, int32_t backward, size_t* out);
+int issm_gated_scan_fwd(const issm_gated_scan_args* args);
+int issm_gated_scan_bwd(const issm_gated_scan_args* args);
+
+/* One token of `rows` sequences: x, gate, in_gate (rows, C) with element strides between rows, y (rows, C) contiguous, state (slots, C) fp32 with
+ * state_stride >= C between slots, updated in place.  slots_of (rows) int32 or int64 (slots_64) names each row's slot, NULL: row r has slot r.  A row whose slot is
+ * outside [0, slots) gives zeros and touches no state; rows of one slot are taken in their order, as tokens one behind the other. */
+typedef struct issm_gated_scan_step_args {
+  int32_t rows, channels;
+  int64_t slots;
+  int32_t dtype;
+  uint32_t flags;
+  const void* x;
+  const void* gate;
+  const void* in_gate; /* optional */
+  int64_t x_stride, gate_stride, in_gate_stride;
+  const float* A;
+  float* state;
+  int64_t state_stride;
+  const void* slots_of; /* optional */
+  int32_t slots_64;
+  void* y;
+  void* stream;
+} issm_gated_scan_step_args;
+
+int issm_gated_scan_step(const issm_gated_scan_step_args* args);
+
+/* ---- rotary positions, with or without the norm of each head ---------------------------------
+ * For one or two sides (queries, keys) of `heads[i]` heads (0: absent) of `headdim` features:
+ *   v = x / sqrt(mean(x^2) + eps) w   (issm_rotary_norm_*; x itself in issm_rotary)
+ *   y1 = v1 c - v2 s,  y2 = v1 s + v2 c   for the pairs (j, j + rot / 2), ISSM_ROT_INTERLEAVED (2j, 2j + 1), of the first `rot` features;
+ * c and s from row `position` of table (table_rows, rot) fp32 contiguous: rot / 2 cosines, then as many sines.  positions (B, L) int32 or int64
+ * (positions_64) with element strides (0 repeats) or NULL: a token's place in its sequence (seqlen <= table_rows then).  The turned features of
+ * a position outside the table are NaN.  x, dy (B, L, H, D) in `dtype`, features contiguous, element strides of batch, token and head; y, dx
+ * (B, L, H, D) contiguous.  w, dw (D) in weight_dtype.  ISSM_ROT_BACK turns the other way: issm_rotary's backward.  issm_rotary_norm_bwd's scratch:
+ * issm_rotary_norm_bwd_bytes; dw[i] NULL = not wanted.  headdim <= 1024, rot even and >= 2, tokens times heads below 2^31. */
+#define ISSM_ROT_INTERLEAVED 1u
+#define ISSM_ROT_BACK 2u
+typedef struct issm_rotary_args {
+  int32_t batch, seqlen, headdim, rot;
+  int32_t heads[2];
+  int32_t dtype, weight_dtype;
+  uint32_t flags;
+  float eps;
+  const void* x[2];
+  int64_t x_stride[2][3];
+  const void* w[2];
+  void* y[2];
+  const float* table;
+  int64_t table_rows;
+  const void* positions;
+  int64_t positions_stride[2];
+  int32_t positions_64;
+  /* backward of the norm */
+  const void* dy[2];
+  int64_t dy_stride[2][3];
+  void* dx[2];
+  void* dw[2];
+  void* scratch;
+  size_t scratch_bytes;
+  void* stream;
+} issm_rotary_args;
+
+int issm_rotary(const issm_rotary_args* args);
+int issm_rotary_norm_fwd(const issm_rotary_args* args);
+int issm_rotary_norm_bwd_bytes(const issm_rotary_args* args, size_t* out);
+int issm_rotary_norm_bwd(const issm_rotary_args* args);
+
 #ifdef __cplusplus
 }
 #endif

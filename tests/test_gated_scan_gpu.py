@@ -1,0 +1,421 @@
+"""gated_scan and gated_scan_step against the recurrence token by token in float64 (oracle/sequence_ref.py)."""
+import pytest
+import torch
+
+from oracle import sequence_ref as R
+
+pytestmark = pytest.mark.gpu
+
+# A step of the recurrence rounds its decay and its state once each in fp32, 2^-24 of the state at most, and takes beta from a reciprocal, a
+# series and a root of about two places each.  The tests' decays remember at most some 60 tokens on average (A <= -0.03 at a gate of 1/2), so that
+# a state is off by 60 * 2 * 2^-24 = 7e-6 of itself if all errors agree; gradients go through two such recurrences.
+FP32 = dict(y=1e-5, grad=2e-5)
+# bf16 results are rounded once on top: half of a step of 2^-7, off by at most 2^-8 of each value and so of their norm (a single value close
+# above a power of two reaches it)
+STEP = 2.0 ** -8
+
+
+def make(B, L, C, dtype, seed=0, in_gate=True, initial=True, packed=0, A_lo=-1.0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    d = dict(x=n(B, L, C).to(dtype), gate=n(B, L, C).to(dtype), A=A_lo + (-0.03 - A_lo) * torch.rand(C, generator=g),
+             in_gate=n(B, L, C).to(dtype) if in_gate else None, initial_states=n(B, C) if initial else None, seq_idx=None)
+    if packed:
+        ids = torch.zeros(B, L, dtype=torch.long)
+        for b in range(B):
+            for c in torch.randint(0, L, (packed,), generator=g).tolist():
+                ids[b, c:] += 1
+        ids[0] -= ids[0, 0].clone()    # one row that takes its initial states
+        d["seq_idx"] = ids
+    return d, n(B, L, C).to(dtype), n(B, C)
+
+
+LEAVES = ("x", "gate", "A", "in_gate", "initial_states")
+
+
+def run(d, dy, dlast, **kw):
+    from dest3d_amd import gated_scan
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    for k in LEAVES:
+        if g[k] is not None:
+            g[k].requires_grad_()
+    y, last = gated_scan(**g, return_final_states=True, **kw)
+    names = [k for k in LEAVES if g[k] is not None]
+    grads = torch.autograd.grad((y, last), [g[k] for k in names], (dy.cuda(), dlast.cuda()))
+    return dict(y=y.detach(), last=last.detach(), **{"d" + k: v for k, v in zip(names, grads)})
+
+
+def ref(d, dy, dlast, **kw):
+    r = {k: v if v is None or k == "seq_idx" else v.double().requires_grad_() for k, v in d.items()}
+    y, last = R.gated_scan(**r, **kw)
+    names = [k for k in LEAVES if r[k] is not None]
+    grads = torch.autograd.grad((y, last), [r[k] for k in names], (dy.double(), dlast.double()), allow_unused=True)
+    return dict(y=y.detach(), last=last.detach(), **{"d" + k: torch.zeros_like(r[k]) if v is None else v for k, v in zip(names, grads)})
+
+
+def check(got, want):
+    for k, w in want.items():
+        v = got[k].double().cpu()
+        assert v.shape == w.shape and torch.isfinite(v).all(), k
+        lim = FP32["grad" if k.startswith("d") else "y"] + (STEP if got[k].dtype == torch.bfloat16 else 0.0)
+        off, size = (v - w).norm().item(), w.norm().item()
+        assert off <= lim * size + 1e-30, (k, off / max(size, 1e-300), lim)
+
+
+SIZES = [(1, 1, 1), (2, 1, 5), (3, 2, 3), (1, 127, 4), (2, 128, 64), (3, 129, 65), (2, 300, 70), (1, 513, 130), (2, 1000, 288), (1, 2049, 67)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C", SIZES)
+def test_forward_and_gradients(B, L, C, dtype):
+    case = make(B, L, C, dtype, seed=L + C)
+    check(run(*case), ref(*case))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("in_gate,normalize,initial,packed,reverse", [
+    (False, True, True, 0, False), (True, False, True, 0, False), (False, False, False, 0, False), (True, True, False, 5, False),
+    (True, True, True, 9, True), (False, False, True, 4, True), (False, True, True, 3, False), (True, False, False, 12, False),
+    (True, True, True, 0, True)])
+def test_forms(in_gate, normalize, initial, packed, reverse, dtype):
+    for B, L, C in ((2, 333, 40), (2, 37, 2)):
+        case = make(B, L, C, dtype, seed=packed, in_gate=in_gate, initial=initial, packed=packed)
+        check(run(*case, normalize=normalize, reverse=reverse), ref(*case, normalize=normalize, reverse=reverse))
+
+
+def test_every_token_a_sequence_of_its_own():
+    case = make(2, 300, 24, torch.float32)
+    case[0]["seq_idx"] = torch.arange(300).expand(2, 300).clone()
+    check(run(*case), ref(*case))
+    case[0]["seq_idx"] = torch.arange(1, 301).expand(2, 300).clone()   # (and none that takes the initial states)
+    got = run(*case)
+    check(got, ref(*case))
+    assert not got["dinitial_states"].any()
+
+
+def test_one_sequence_by_name_is_no_packing():
+    d, dy, dlast = make(2, 300, 24, torch.float32)
+    plain = run(d, dy, dlast)
+    named = run(dict(d, seq_idx=torch.zeros(2, 300, dtype=torch.int32)), dy, dlast)
+    assert all(torch.equal(plain[k], named[k]) for k in plain)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides(dtype):
+    """Slices of one projection at odd offsets, rows in another order, repeated inputs: as their contiguous copies, bit for bit."""
+    from dest3d_amd import gated_scan
+    g = torch.Generator().manual_seed(3)
+    B, L, C = 2, 260, 70
+    wide = torch.randn(L, B, 3 * C + 5, generator=g).to(dtype).cuda()
+    x, gate, in_gate = (wide[..., 1 + i * (C + 1):1 + i * (C + 1) + C].transpose(0, 1) for i in range(3))
+    A = -torch.rand(C, generator=g).cuda() - 0.03
+    repeated = torch.randn(1, 1, C, generator=g).to(dtype).cuda().expand(B, L, C)
+    ids = (torch.arange(L, dtype=torch.int32) // 50)[None].expand(B, L).cuda()
+    for kw in (dict(gate=gate, in_gate=in_gate), dict(gate=repeated, in_gate=in_gate), dict(gate=gate, in_gate=repeated)):
+        for reverse in (False, True):
+            a = gated_scan(x, A=A, seq_idx=ids, reverse=reverse, **kw)
+            b = gated_scan(x.contiguous(), A=A, seq_idx=ids.contiguous(), reverse=reverse, **{k: v.contiguous() for k, v in kw.items()})
+            assert torch.equal(a, b)
+    # a gradient that is repeated, and those of a repeated input and of channels that are not contiguous
+    xr = torch.randn(B, 1, C, generator=g).to(dtype).cuda().requires_grad_()
+    xt = torch.randn(B, C, L, generator=g).to(dtype).cuda().requires_grad_()
+    gated_scan(xr.expand(B, L, C) + xt.transpose(1, 2), gate, A).sum().backward()
+    full = (xr.detach().expand(B, L, C) + xt.detach().transpose(1, 2)).contiguous().requires_grad_()
+    gated_scan(full, gate, A).backward(torch.ones_like(full))
+    assert torch.equal(xt.grad, full.grad.transpose(1, 2))
+    assert torch.equal(xr.grad, full.grad.sum(1, keepdim=True))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_nothing_passes_a_cut(bad, reverse):
+    """A sequence whose inputs, states or gradients are no numbers leaves its neighbours' results and gradients as they were."""
+    d, dy, dlast = make(2, 300, 24, torch.float32)
+    ids = torch.zeros(2, 300, dtype=torch.int32)
+    ids[:, 90:170], ids[:, 170:] = 1, 2
+    d["seq_idx"] = ids
+    clean = run(d, dy, dlast, reverse=reverse)
+    for where in ("x", "gate", "in_gate", "dy"):
+        e, ey = {k: None if v is None else v.clone() for k, v in d.items()}, dy.clone()
+        (ey if where == "dy" else e[where])[:, 120] = bad
+        got = run(e, ey, dlast, reverse=reverse)
+        keep = torch.ones(300, dtype=torch.bool)
+        keep[90:170] = False
+        for k in ("y", "dx", "dgate", "din_gate"):
+            assert torch.equal(got[k][:, keep], clean[k][:, keep]), (where, k)
+        assert torch.equal(got["last"], clean["last"]) and torch.equal(got["dinitial_states"], clean["dinitial_states"])
+        if where == "x" and bad != bad:
+            assert torch.isnan(got["y"][:, 120]).all()
+
+
+def test_gates_at_their_ends():
+    """Full and empty gates, infinite ones too, and channels that nothing decays in: values as the formula's limits, gradients finite."""
+    B, L, C = 1, 140, 8
+    d, dy, dlast = make(B, L, C, torch.float32)
+    d["gate"][:, ::3] = 60.0
+    d["gate"][:, 1::3] = -60.0
+    d["gate"][:, 7], d["gate"][:, 8] = -float("inf"), float("inf")
+    d["in_gate"][:, ::5] = -200.0
+    want = ref(dict(d, gate=d["gate"].clamp(-300, 300)), dy, dlast)
+    got = run(d, dy, dlast)
+    # where beta is 0 (sigmoid(-300) = 5e-131 rounds to it in fp32) the oracle in float64 still has a number, below 1e-60
+    check(got, want)
+    d["A"][:4] = 0.0
+    got = run(d, dy, dlast)
+    assert all(torch.isfinite(v).all() for v in got.values())
+    want = d["initial_states"][:, None, :4].expand(B, L, 4)
+    assert torch.equal(got["y"][..., :4].cpu(), want)
+    assert not got["dgate"][..., :4].any()
+    # a state that stays: dA is what the decays' own part gives, sum c_t h_{t-1} r_t, and nothing through beta, whose derivative has no value there
+    c = dy[..., :4].double().flip(1).cumsum(1).flip(1) + dlast[:, None, :4].double()
+    terms = c * want.double() * torch.sigmoid(d["gate"][..., :4].double())
+    assert ((got["dA"][:4].double().cpu() - terms.sum((0, 1))).abs() <= FP32["grad"] * terms.abs().sum((0, 1))).all()
+
+
+def test_decays_of_all_sizes():
+    """From nothing to far beyond fp32's range, on both sides of the series' end, over a length that a decay next to one remembers whole."""
+    B, L, C = 1, 600, 16
+    d, dy, dlast = make(B, L, C, torch.float32)
+    d["A"] = -torch.logspace(-6, 4, C)
+    d["gate"] = torch.randn(B, L, C, generator=torch.Generator().manual_seed(1))
+    got, want = run(d, dy, dlast), ref(d, dy, dlast)
+    for c in range(C):   # each channel by itself: 600 steps of 2^-24 twice, if all errors agree, in a gradient twice that
+        for k in want:
+            if k == "dA":
+                continue   # (its terms cancel in channels that remember all: below, by its own terms' size)
+            v, w = got[k][..., c].double().cpu(), want[k][..., c]
+            assert (v - w).norm() <= (1.5e-4 if k.startswith("d") else 7.2e-5) * w.norm() + 1e-30, (c, k)
+    r = {k: v if v is None or k == "seq_idx" else v.double() for k, v in d.items()}
+    A = r["A"][None].expand(L, C).clone().requires_grad_()   # a parameter for each token: the terms of dA
+    y, last = R.gated_scan(r["x"], r["gate"], A[None], r["in_gate"], r["initial_states"])
+    (terms,) = torch.autograd.grad((y, last), (A,), (dy.double(), dlast.double()))
+    assert ((got["dA"].double().cpu() - want["dA"]).abs() <= 1.5e-4 * terms.abs().sum(0) + 1e-30).all()
+
+
+def test_gradients_by_differences():
+    from dest3d_amd import gated_scan
+    d, dy, dlast = make(2, 150, 9, torch.float32, packed=2)
+    got = run(d, dy, dlast)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+
+    def loss(**kw):
+        y, last = gated_scan(**{**g, **kw}, return_final_states=True)
+        return (y.double() * dy.cuda().double()).sum() + (last.double() * dlast.cuda().double()).sum()
+
+    gen = torch.Generator().manual_seed(5)
+    for k in LEAVES:
+        v = torch.randn(g[k].shape, generator=gen).cuda()
+        if k == "A":
+            v = v * 0.02      # (A stays below 0)
+        v = torch.sign((got["d" + k] * v).sum()) * v + 0.3 * got["d" + k] / got["d" + k].abs().max() * v.abs().mean()   # (a direction with a slope)
+        e = 2.0 ** -6
+        slope = (loss(**{k: g[k] + e * v}) - loss(**{k: g[k] - e * v})).item() / (2 * e)
+        want = (got["d" + k].double() * v.double()).sum().item()
+        # the third derivative's share, e^2 / 6 of a function of exponentials of unit scale, and fp32 results' 1e-5 of the loss's terms over 2 e
+        assert abs(slope - want) <= 2e-2 * abs(want), (k, slope, want)
+
+
+def test_other_types():
+    from dest3d_amd import gated_scan
+    d, dy, dlast = make(2, 100, 12, torch.float32)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    base = gated_scan(**g)
+    for t in (torch.float16, torch.float64):
+        e = {k: v if v is None else v.to(t) for k, v in g.items()}
+        y, last = gated_scan(**e, return_final_states=True)
+        assert y.dtype == t and last.dtype == torch.float32
+        torch.testing.assert_close(y.float(), base, rtol=2e-2, atol=2e-2) if t == torch.float16 else torch.testing.assert_close(y.float(), base, rtol=0, atol=0)
+    x = g["x"].to(torch.bfloat16).requires_grad_()
+    gate, A = g["gate"].requires_grad_(), g["A"].to(torch.float64).requires_grad_()
+    y = gated_scan(x, gate, A)
+    y.float().sum().backward()
+    assert (y.dtype, x.grad.dtype, gate.grad.dtype, A.grad.dtype) == (torch.bfloat16, torch.bfloat16, torch.float32, torch.float64)
+
+
+def test_no_tokens_and_no_rows():
+    from dest3d_amd import gated_scan, gated_scan_step
+    for B, L, C in ((2, 0, 5), (0, 4, 5), (2, 4, 0)):
+        x = torch.zeros(B, L, C, device="cuda", requires_grad=True)
+        A, h0 = torch.full((C,), -1.0, device="cuda", requires_grad=True), torch.randn(B, C, device="cuda", requires_grad=True)
+        y, last = gated_scan(x, x, A, initial_states=h0, return_final_states=True)
+        assert y.shape == x.shape and last.shape == (B, C)
+        if L == 0:
+            assert torch.equal(last, h0)
+        w = torch.randn(B, C, device="cuda")
+        (y.sum() + (last * w).sum()).backward()
+        assert x.grad.shape == x.shape and not A.grad.any()
+        if L == 0:
+            assert torch.equal(h0.grad, w)
+        assert torch.equal(gated_scan(x.detach(), x.detach(), A.detach(), return_final_states=True)[1], h0 * 0)
+    x = torch.zeros(0, 5, device="cuda")
+    assert gated_scan_step(x, x, torch.full((5,), -1.0, device="cuda"), torch.zeros(0, 5, device="cuda")).shape == (0, 5)
+
+
+def test_parts_of_the_gradients():
+    """Only what is asked for, and with either gradient of the results absent: as in the whole, bit for bit."""
+    from dest3d_amd import gated_scan
+    d, dy, dlast = make(2, 140, 20, torch.bfloat16)
+    whole = run(d, dy, torch.zeros_like(dlast))
+    for k in LEAVES:
+        g = {n: None if v is None else v.cuda() for n, v in d.items()}
+        g[k].requires_grad_()
+        (grad,) = torch.autograd.grad(gated_scan(**g), (g[k],), (dy.cuda(),))
+        assert torch.equal(grad, whole["d" + k]), k
+    g = {n: None if v is None else v.cuda() for n, v in d.items()}
+    g["x"].requires_grad_()
+    _, last = gated_scan(**g, return_final_states=True)
+    (grad,) = torch.autograd.grad(last, (g["x"],), (dlast.cuda(),))
+    assert torch.equal(grad, run(d, torch.zeros_like(dy), dlast)["dx"])
+
+
+def test_same_bits_twice_and_without_gradients():
+    from dest3d_amd import gated_scan
+    d, dy, dlast = make(3, 700, 100, torch.bfloat16, packed=3)
+    a, b = run(d, dy, dlast), run(d, dy, dlast)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+    with torch.no_grad():
+        y, last = gated_scan(**{k: None if v is None else v.cuda() for k, v in d.items()}, return_final_states=True)
+    assert torch.equal(y, a["y"]) and torch.equal(last, a["last"])
+
+
+def test_streams():
+    """Two calls at once, on streams of their own."""
+    from dest3d_amd import gated_scan
+    cases = [make(2, 3000, 96, torch.float32, seed=s) for s in (1, 2)]
+    want = [run(*c) for c in cases]
+    g = [{k: None if v is None else v.cuda() for k, v in c[0].items()} for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(gated_scan(**g[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]["y"]) for i in range(2) for y in got[i])
+
+
+def test_captured():
+    """Forward and backward in a graph, replayed on other inputs with eager work between the replays; two graphs at once."""
+    from dest3d_amd import gated_scan
+    graphs = []
+    for seed, L in ((1, 700), (2, 90)):
+        d, dy, dlast = make(2, L, 72, torch.float32, seed=seed)
+        g = {k: None if v is None else v.cuda() for k, v in d.items()}
+        for k in LEAVES:
+            g[k].requires_grad_()
+        dyg = dy.cuda()
+
+        def step(g=g, dyg=dyg):
+            y = gated_scan(**g)
+            return [y.detach(), *torch.autograd.grad(y, [g[k] for k in LEAVES], (dyg,))]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, g, step, out))
+    for turn in range(3):
+        for graph, g, step, out in graphs:
+            with torch.no_grad():
+                for k in LEAVES:
+                    g[k].add_(0.01 * turn * torch.randn_like(g[k])) if k != "A" else g[k].mul_(1.01)
+            want = step()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_backward_reads_its_inputs_as_they_were():
+    from dest3d_amd import gated_scan
+    d, dy, _ = make(1, 50, 8, torch.float32)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    x = g["x"].requires_grad_() * 1.0
+    y = gated_scan(x, g["gate"], g["A"])
+    x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy.cuda())
+    x = g["x"].detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(gated_scan(x, g["gate"], g["A"]).sum(), x, create_graph=True)
+
+
+# ------------------------------------------------------------------------------------------------------------ one token
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C,in_gate,normalize", [(1, 1, True, True), (3, 7, False, True), (5, 288, True, False), (2, 1030, True, True), (70, 64, False, False)])
+def test_step_by_step_is_the_scan(rows, C, in_gate, normalize, dtype):
+    from dest3d_amd import gated_scan_step
+    d, _, _ = make(rows, 6, C, dtype, seed=C, in_gate=in_gate)
+    want, last = R.gated_scan(**{k: v if v is None else v.double() for k, v in d.items()}, normalize=normalize)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    state = g["initial_states"].clone()
+    for t in range(6):
+        y = gated_scan_step(g["x"][:, t], g["gate"][:, t], g["A"], state, in_gate=None if g["in_gate"] is None else g["in_gate"][:, t], normalize=normalize)
+        lim = 1e-5 + (STEP if dtype == torch.bfloat16 else 0.0)
+        assert y.dtype == dtype and ((y.double().cpu() - want[:, t]).abs() <= lim * want[:, t].abs() + 1e-5).all()
+    assert ((state.double().cpu() - last).abs() <= 1e-5 * last.abs() + 1e-5).all()
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_step_in_a_pool(index):
+    """Slots in any order, rows without one, one slot several times, and a pool whose slots lie apart."""
+    from dest3d_amd import gated_scan_step
+    rows, C, slots = 150, 37, 40
+    d, _, _ = make(1, rows, C, torch.float32)
+    g = {k: None if v is None else v[0].cuda() if v.dim() > 1 else v.cuda() for k, v in d.items()}
+    gen = torch.Generator().manual_seed(2)
+    wide = torch.randn(slots, C + 11, generator=gen).cuda()
+    before = wide.clone()
+    at = torch.randint(-2, slots + 3, (rows,), generator=gen)
+    at[5], at[6], at[149] = 7, 7, 7
+    if index == torch.int64:
+        at[9] = 2 ** 32 + 3    # (no slot, whatever its low half says)
+    y = gated_scan_step(g["x"], g["gate"], g["A"], wide[:, 3:3 + C], in_gate=g["in_gate"], state_indices=at.to(index).cuda())
+    state = before[:, 3:3 + C].double().cpu()
+    for r in range(rows):
+        s = int(at[r])
+        if not 0 <= s < slots:
+            assert not y[r].any()
+            continue
+        one = lambda t: t[r].double().cpu()[None, None]  # noqa: E731
+        h, _ = R.gated_scan(one(g["x"]), one(g["gate"]), g["A"].double().cpu(), one(g["in_gate"]), state[s][None].clone())
+        state[s] = h[0, 0]
+        assert ((y[r].double().cpu() - h[0, 0]).abs() <= 2e-5).all(), r
+    assert ((wide[:, 3:3 + C].double().cpu() - state).abs() <= 2e-5).all()
+    assert torch.equal(wide[:, :3], before[:, :3]) and torch.equal(wide[:, 3 + C:], before[:, 3 + C:])
+    touched = torch.zeros(slots, dtype=torch.bool)
+    touched[at[(at >= 0) & (at < slots)]] = True
+    assert torch.equal(wide[~touched.cuda()], before[~touched.cuda()])
+
+
+def test_step_tells_what_saved_its_state_and_is_captured():
+    from dest3d_amd import gated_scan_step
+    d, _, _ = make(1, 4, 8, torch.float32)
+    g = {k: None if v is None else v[0].cuda() if v.dim() > 1 else v.cuda() for k, v in d.items()}
+    state = torch.randn(4, 8, device="cuda")
+    version = state._version
+    w = torch.ones(4, 8, device="cuda", requires_grad=True)
+    kept = (w * state).sum()
+    gated_scan_step(g["x"], g["gate"], g["A"], state)
+    assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    at = torch.tensor([2, 0, -1, 3], device="cuda")
+    y0 = gated_scan_step(g["x"], g["gate"], g["A"], state.clone(), state_indices=at)
+    graph = torch.cuda.CUDAGraph()
+    start = state.clone()
+    with torch.cuda.graph(graph):
+        y = gated_scan_step(g["x"], g["gate"], g["A"], state, state_indices=at)
+    for _ in range(3):
+        state.copy_(start)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, y0)
+    with torch.inference_mode():
+        gated_scan_step(g["x"], g["gate"], g["A"], torch.zeros(4, 8, device="cuda"))
