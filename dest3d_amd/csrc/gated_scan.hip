@@ -69,19 +69,70 @@ __device__ __forceinline__ void tile_starts(const float (&sP)[TT][W], float (&sH
   }
 }
 
-template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ>
+// The state in front of the o-th tile of a row (in the order of the walk), a channel a lane, from what the tiles in front of it have told:
+// the nearest state among the last GS_LOOK of them, and the maps from there on, in the order in which the tiles themselves apply
+// them -- whichever of the states is found, the bits are the same.
+// Every wait ends: tiles are taken in their order (tickets), so the tiles in front of this one are on workgroups that run, and the first of them
+// that has not told its state waits for none that has not.  (After GS_POLLS looks, seconds, it would end with NaN: should memory be overwritten
+// from elsewhere, no workgroup stays.)
+constexpr int GS_LOOK = 8, GS_POLLS = 1 << 22;
+__device__ __forceinline__ float look_back(const unsigned long long* words, int o, float first, int lane) {
+  float H[GS_LOOK], P[GS_LOOK];
+  int n = GS_LOOK;
+  for (int polls = 0; polls < GS_POLLS; ++polls) {
+    unsigned long long w[GS_LOOK];
+#pragma unroll
+    for (int i = 0; i < GS_LOOK; ++i)
+      w[i] = __hip_atomic_load(words + (long)max(o - 1 - i, 0) * 64 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    n = GS_LOOK;
+    bool told = true;
+#pragma unroll
+    for (int i = 0; i < GS_LOOK; ++i) {
+      unsigned high = (unsigned)(w[i] >> 32);
+      H[i] = __uint_as_float((unsigned)w[i]);
+      if (o - 1 - i < 0) {   // in front of the first: the state that the row starts from
+        high = GS_STATE;
+        H[i] = first;
+      }
+      P[i] = __uint_as_float(high);
+      if (told && n == GS_LOOK && high == GS_STATE) n = i;
+      told = told && high != GS_NOTHING;
+    }
+    if (__all(n < GS_LOOK)) break;
+    __builtin_amdgcn_s_sleep(2);
+  }
+  float h = __builtin_nanf("");
+#pragma unroll
+  for (int i = GS_LOOK - 1; i >= 0; --i) h = i == n ? H[i] : i < n ? fmaf(P[i], h, H[i]) : h;
+  return h;
+}
+// The tile's ticket; one barrier
+__device__ __forceinline__ int ticket(unsigned* counter, int* shared) {
+  if (threadIdx.x == 0) *shared = (int)(__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u);
+  __syncthreads();
+  return *shared;
+}
+__global__ __launch_bounds__(256) void k_gscan_clear(uint4* p, long n) {
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+}
+
+// LOOK: a tile a workgroup; else a row's tiles one behind the other on one
+template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ, bool LOOK>
 __global__ __launch_bounds__(GS_THREADS) void k_gscan_fwd(GScanP p) {
   constexpr int TT = GS_TT, W = GS_CG * V, T = TT * S;
   __shared__ float sP[TT][W], sH[TT][W];
   const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG;
-  const int cb = blockIdx.x % p.ncb, b = blockIdx.x / p.ncb;
+  const int chain = LOOK ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
   const int c0 = first_channel<V>(cb * W + cg * V, p.C), mine = slot_channel<V>(cb * W, tid, p.C);
   float A[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) A[v] = p.A[c0 + v];
   float carry = 0.0f;
   if (tid < W && p.h0) carry = p.h0[(long)b * p.C + mine];
-  for (int k = 0; k < p.nk; ++k) {
+  __shared__ int turn;
+  const int k0 = LOOK ? ticket(p.tickets + (long)chain * GS_TICKET, &turn) : 0, k1 = LOOK ? k0 + 1 : p.nk;
+  unsigned long long* words = p.words + (long)chain * p.nk * 64;
+  for (int k = k0; k < k1; ++k) {
     const int t0 = k * T + tt * S;
     Raw<BF, V, S> x, g, in;
     x.load(p.x, p.xb, p.xl, b, t0, c0, p.L - 1);
@@ -131,9 +182,16 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_fwd(GScanP p) {
     if (tid < W) {
       float Pt, Ht;
       tile_map<SEQ, TT, W>(sP, sH, tid, false, Pt, Ht);
+      if (LOOK && k > 0) {
+        const bool cut_off = SEQ && Pt < 0.0f;
+        tell(words + (long)k * 64 + tid, Ht, cut_off ? GS_STATE : map_bits(Pt));
+        carry = look_back(words, k, carry, tid);
+      }
       if (p.hs) p.hs[((long)b * p.nk + k) * p.C + mine] = carry;
+      const float behind = SEQ && Pt < 0.0f ? Ht : fmaf(Pt, carry, Ht);
+      if (LOOK && k + 1 < p.nk) tell(words + (long)k * 64 + tid, behind, GS_STATE);
       tile_starts<SEQ, TT, W>(sP, sH, tid, false, carry);
-      carry = SEQ && Pt < 0.0f ? Ht : fmaf(Pt, carry, Ht);
+      carry = behind;
     }
     __syncthreads();
     float h[V];
@@ -147,16 +205,16 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_fwd(GScanP p) {
       if (t < p.L) Piece<BF, V>::store(p.y, b * p.yb + t * p.yl + c0, h);
       if (t == p.L - 1 && p.last) Piece<false, V>::store(p.last, (long)b * p.C + c0, h);
     }
-    __syncthreads();   // (the next tile's maps go where these states are read)
+    if (!LOOK) __syncthreads();   // (the next tile's maps go where these states are read)
   }
 }
 
-template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ>
+template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ, bool LOOK>
 __global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
   constexpr int TT = GS_TT, W = GS_CG * V, T = TT * S;
   __shared__ float sP[TT][W], sH[TT][W], sC[TT][W];
   const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG;
-  const int cb = blockIdx.x % p.ncb, b = blockIdx.x / p.ncb;
+  const int chain = LOOK ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
   const int c0 = first_channel<V>(cb * W + cg * V, p.C), mine = slot_channel<V>(cb * W, tid, p.C);
   float A[V], dA[V];
 #pragma unroll
@@ -166,7 +224,11 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
   }
   float carry = 0.0f;   // what the tokens behind the tile give to its last state
   if (tid < W && p.dlast) carry = p.dlast[(long)b * p.C + mine];
-  for (int k = p.nk - 1; k >= 0; --k) {
+  __shared__ int turn;
+  const int o0 = LOOK ? ticket(p.tickets + (long)chain * GS_TICKET, &turn) : 0, o1 = LOOK ? o0 + 1 : p.nk;
+  unsigned long long* words = p.words + (long)chain * p.nk * 64;
+  for (int o = o0; o < o1; ++o) {   // from the last tile to the first
+    const int k = p.nk - 1 - o;
     const int t0 = k * T + tt * S;
     Raw<BF, V, S> x, g, in, dy;
     x.load(p.x, p.xb, p.xl, b, t0, c0, p.L - 1);
@@ -222,10 +284,17 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
     __syncthreads();
     if (tid < W) {
       float Pt, Ct;
+      const float before = p.hs[((long)b * p.nk + k) * p.C + mine];
       tile_map<SEQ, TT, W>(sP, sC, tid, true, Pt, Ct);
-      tile_starts<SEQ, TT, W>(sP, sH, tid, false, p.hs[((long)b * p.nk + k) * p.C + mine]);
+      if (LOOK && o > 0) {
+        tell(words + (long)o * 64 + tid, Ct, SEQ && Pt < 0.0f ? GS_STATE : map_bits(Pt));
+        carry = look_back(words, o, carry, tid);
+      }
+      const float behind = SEQ && Pt < 0.0f ? Ct : fmaf(Pt, carry, Ct);
+      if (LOOK && o + 1 < p.nk) tell(words + (long)o * 64 + tid, behind, GS_STATE);
       tile_starts<SEQ, TT, W>(sP, sC, tid, true, carry);
-      carry = SEQ && Pt < 0.0f ? Ct : fmaf(Pt, carry, Ct);
+      tile_starts<SEQ, TT, W>(sP, sH, tid, false, before);
+      carry = behind;
     }
     __syncthreads();
     float h[V], c[V];
@@ -275,9 +344,10 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
       }
       if (t == 0 && p.dh0) Piece<false, V>::store(p.dh0, (long)b * p.C + c0, c);
     }
-    __syncthreads();
+    if (!LOOK) __syncthreads();
   }
   if (!p.part) return;
+  if (LOOK) __syncthreads();
 #pragma unroll
   for (int v = 0; v < V; ++v) sP[tt][cg * V + v] = dA[v];
   __syncthreads();
@@ -285,20 +355,24 @@ __global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
     float sum = 0.0f;
 #pragma unroll 8
     for (int j = 0; j < TT; ++j) sum += sP[j][tid];
-    p.part[(long)b * p.C + mine] = sum;
+    p.part[((long)b * (LOOK ? p.nk : 1) + (LOOK ? p.nk - 1 - o0 : 0)) * p.C + mine] = sum;
   }
 }
 
 // dA: the sums of `rows` partial rows, in their order
-__global__ __launch_bounds__(256) void k_gscan_sum(const float* part, int rows, int C, float* out) {
-  __shared__ float s[4][64];
+__global__ __launch_bounds__(1024) void k_gscan_sum(const float* part, int rows, int C, float* out) {
+  __shared__ float s[16][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   float sum = 0.0f;
   if (c < C)
-    for (int r = wv; r < rows; r += 4) sum += part[(long)r * C + c];
+    for (int r = wv; r < rows; r += 16) sum += part[(long)r * C + c];
   s[wv][lane] = sum;
   __syncthreads();
-  if (wv == 0 && c < C) out[c] = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+  if (wv || c >= C) return;
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum += s[i][lane];
+  out[c] = sum;
 }
 
 // One token a row.  Rows whose slot is none of the pool's give zeros and touch no state.  Several rows of one slot are taken in their order, by
@@ -350,30 +424,59 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
     if (v < n) state[c0 + v] = h[v];
 }
 
-template <bool BF, int V, bool IG, bool NRM>
+template <bool BF, int V, bool IG, bool NRM, bool SEQ>
 static void launch_dir(const GScanP& p, bool back, int blocks, hipStream_t st) {
   if (back) {
-    if (p.ids) k_gscan_bwd<BF, V, GS_S, IG, NRM, true><<<blocks, GS_THREADS, 0, st>>>(p);
-    else k_gscan_bwd<BF, V, GS_S, IG, NRM, false><<<blocks, GS_THREADS, 0, st>>>(p);
+    if (p.words) k_gscan_bwd<BF, V, GS_S, IG, NRM, SEQ, true><<<blocks, GS_THREADS, 0, st>>>(p);
+    else k_gscan_bwd<BF, V, GS_S, IG, NRM, SEQ, false><<<blocks, GS_THREADS, 0, st>>>(p);
   } else {
-    if (p.ids) k_gscan_fwd<BF, V, GS_S, IG, NRM, true><<<blocks, GS_THREADS, 0, st>>>(p);
-    else k_gscan_fwd<BF, V, GS_S, IG, NRM, false><<<blocks, GS_THREADS, 0, st>>>(p);
+    if (p.words) k_gscan_fwd<BF, V, GS_S, IG, NRM, SEQ, true><<<blocks, GS_THREADS, 0, st>>>(p);
+    else k_gscan_fwd<BF, V, GS_S, IG, NRM, SEQ, false><<<blocks, GS_THREADS, 0, st>>>(p);
   }
+}
+template <bool BF, int V, bool IG, bool NRM>
+static void launch_packed(const GScanP& p, bool back, int blocks, hipStream_t st) {
+  p.ids ? launch_dir<BF, V, IG, NRM, true>(p, back, blocks, st) : launch_dir<BF, V, IG, NRM, false>(p, back, blocks, st);
 }
 template <bool BF, int V>
 static void launch_form(const GScanP& p, bool nrm, bool back, int blocks, hipStream_t st) {
-  if (p.i) return nrm ? launch_dir<BF, V, true, true>(p, back, blocks, st) : launch_dir<BF, V, true, false>(p, back, blocks, st);
-  return nrm ? launch_dir<BF, V, false, true>(p, back, blocks, st) : launch_dir<BF, V, false, false>(p, back, blocks, st);
+  if (p.i) nrm ? launch_packed<BF, V, true, true>(p, back, blocks, st) : launch_packed<BF, V, true, false>(p, back, blocks, st);
+  else nrm ? launch_packed<BF, V, false, true>(p, back, blocks, st) : launch_packed<BF, V, false, false>(p, back, blocks, st);
 }
 
-int launch_gscan(GScanP p, bool bf, bool nrm, bool back, hipStream_t st) {
+// Whether a row's tiles go on workgroups of their own: up to where the rows of blocks of channels fill the GPU twice.  In us, forward and backward,
+// bf16: 256 of them (8 x 4096 x 2048) 140 and 366, walked 169 and 312; 512 (32 x 2048 x 1024) 143 and 371, walked 129 and 315;
+// 32 (1 x 4096 x 2048) 22.5 and 51.5, walked 139 and 254
+bool gscan_looks(int B, int L, int C) { return gscan_tiles(L) > 1 && (long)B * gscan_blocks(C) < 2 * NCU; }
+// Bytes of a call's workspace: partial sums of dA, then the tickets and what the tiles tell, in whole 16 bytes each
+static size_t part_bytes(int B, int L, int C) { return ((size_t)B * (gscan_looks(B, L, C) ? gscan_tiles(L) : 1) * C * 4 + 255) & ~(size_t)255; }
+static size_t ticket_bytes(int B, int C) { return (size_t)B * gscan_blocks(C) * GS_TICKET * 4; }
+static size_t word_bytes(int B, int L, int C) { return (size_t)B * gscan_blocks(C) * gscan_tiles(L) * 64 * 8; }
+size_t gscan_workspace(int B, int L, int C, bool back) {
+  return (back ? part_bytes(B, L, C) : 0) + (gscan_looks(B, L, C) ? ticket_bytes(B, C) + word_bytes(B, L, C) : 0);
+}
+
+int launch_gscan(GScanP p, bool bf, bool nrm, bool back, void* workspace, hipStream_t st) {
   const bool wide = p.C >= 4;
   p.ncb = gscan_blocks(p.C);
   p.nk = gscan_tiles(p.L);
-  const int blocks = p.B * p.ncb;
+  int blocks = p.B * p.ncb, rows = p.B;
+  char* ws = (char*)workspace;
+  if (back) {
+    p.part = p.dA ? (float*)ws : nullptr;
+    ws += part_bytes(p.B, p.L, p.C);
+  }
+  if (gscan_looks(p.B, p.L, p.C)) {
+    p.tickets = (unsigned*)ws;
+    p.words = (unsigned long long*)(ws + ticket_bytes(p.B, p.C));
+    const long n = (long)((ticket_bytes(p.B, p.C) + word_bytes(p.B, p.L, p.C)) / 16);
+    k_gscan_clear<<<(int)min((n + 1023) / 1024, 1024L), 256, 0, st>>>((uint4*)ws, n);
+    blocks *= p.nk;
+    rows *= p.nk;
+  }
   if (bf) wide ? launch_form<true, 4>(p, nrm, back, blocks, st) : launch_form<true, 1>(p, nrm, back, blocks, st);
   else wide ? launch_form<false, 4>(p, nrm, back, blocks, st) : launch_form<false, 1>(p, nrm, back, blocks, st);
-  if (back && p.dA) k_gscan_sum<<<(p.C + 63) / 64, 256, 0, st>>>(p.part, p.B, p.C, p.dA);
+  if (p.part) k_gscan_sum<<<(p.C + 63) / 64, 1024, 0, st>>>(p.part, rows, p.C, p.dA);
   return (int)hipGetLastError();
 }
 

@@ -16,7 +16,20 @@ struct GScanP {
   void *y, *dx, *dg, *di;         // yb, yl: strides of all four
   long yb, yl;
   float *last, *hs, *dh0, *part, *dA;   // (B, C); (B, nk, C) states before the tiles; (B, C); partial sums of dA; (C)
+  unsigned* tickets;              // tiles of a row on workgroups of their own: a counter for each row of a block of channels, GS_TICKET apart, and
+  unsigned long long* words;      // what its tiles tell the ones behind them, (B, ncb, nk, 64); all bits set before the launch
 };
+constexpr int GS_TICKET = 32;
+
+// What a tile tells the ones behind it of a channel, in one access of 8 bytes, so that nothing needs an order of its own: the map of its tokens,
+// H below P, or the state behind it, H below the bits of -0 (P is never negative: a tile with a cut knows the state behind it), or, all bits set,
+// nothing yet.
+constexpr unsigned GS_STATE = 0x80000000u, GS_NOTHING = 0xffffffffu;
+__device__ __forceinline__ void tell(unsigned long long* at, float H, unsigned high) {
+  __hip_atomic_store(at, (unsigned long long)high << 32 | __float_as_uint(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned map_bits(float P) { return P != P ? 0x7fc00000u : __float_as_uint(P); }
+
 struct GStepP {
   int rows, C, ncb;
   long slots, state_s;

@@ -88,7 +88,8 @@ int launch_dwconv_bwd(const DwConvP& p, hipStream_t st);
 int pgen_bwd_blocks(long tokens);
 int launch_pgen_fwd(const PGenP& p, hipStream_t st);
 int launch_pgen_bwd(const PGenP& p, hipStream_t st);
-int launch_gscan(GScanP p, bool bf, bool nrm, bool back, hipStream_t st);
+size_t gscan_workspace(int B, int L, int C, bool back);
+int launch_gscan(GScanP p, bool bf, bool nrm, bool back, void* workspace, hipStream_t st);
 int launch_gscan_step(GStepP p, bool bf, bool nrm, hipStream_t st);
 int launch_rotary(RotP p, bool bf, bool inter, bool norm, hipStream_t st);
 int launch_rotary_norm_bwd(RotP p, bool bf, bool inter, hipStream_t st);
@@ -1451,7 +1452,7 @@ int issm_gated_scan_workspace_bytes(const issm_gated_scan_args* a, int32_t backw
   int rc = gscan_sizes(a);
   if (rc) return rc;
   if (!out) return fail(ISSM_E_NULL, "out is NULL");
-  *out = backward ? (size_t)a->batch * a->channels * sizeof(float) : 0;
+  *out = gscan_workspace(a->batch, a->seqlen, a->channels, backward);
   return ISSM_OK;
 }
 
@@ -1501,14 +1502,13 @@ static int gscan_call(const issm_gated_scan_args* a, bool back) {
     p.dlast = a->dlast;
     p.dh0 = a->dh0;
     p.dA = a->dA;
-    if (need && (!a->workspace || a->workspace_bytes < need))
-      return fail(ISSM_E_WORKSPACE, "gated_scan bwd: %zu bytes of workspace, %zu needed", a->workspace_bytes, need);
-    p.part = a->dA ? (float*)a->workspace : nullptr;
   } else {
     p.y = first(a->y);
     p.last = a->last;
   }
-  return launched(launch_gscan(p, bf, a->flags & ISSM_GS_NORMALIZE, back, (hipStream_t)a->stream), back ? "gated_scan_bwd" : "gated_scan_fwd");
+  if (need && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace & 15))
+    return fail(ISSM_E_WORKSPACE, "gated_scan: %zu bytes of workspace, %zu needed", a->workspace_bytes, need);
+  return launched(launch_gscan(p, bf, a->flags & ISSM_GS_NORMALIZE, back, a->workspace, (hipStream_t)a->stream), back ? "gated_scan_bwd" : "gated_scan_fwd");
 }
 
 int issm_gated_scan_fwd(const issm_gated_scan_args* a) { return gscan_call(a, false); }
