@@ -8,8 +8,9 @@
 // a and beta come from d = 1 - a = -expm1(l): a decay next to one that is rounded with a bias of half a place adds that bias up over
 // all tokens it remembers (1000 at a = 0.999), while 1 - d is rounded to nearest, and 1 - a^2 = d (1 + a) has no cancellation.
 //
-// A workgroup takes tiles of TT * S tokens and CG * V channels: a thread V channels of S tokens one behind the other, whose map
-// h -> P h + H it leaves in LDS; the first wave, a channel a lane, joins the TT maps of the tile and gives every thread its first state.
+// A workgroup takes tiles of GS_TT * S tokens and GS_CG * V channels: a thread V channels of S tokens one behind the other, whose map
+// h -> P h + H it leaves in LDS.  A wave without tokens of its own, a channel a lane, joins the maps of the tile and gives every thread its first
+// state; with the tokens' requests out of its way its looks at other tiles come back at once (a wave's loads return in their order).
 #include "gated_scan_dev.h"
 
 // (every multiply-add is written as one: the forms of a kernel that do the same sums are to give the same bits)
@@ -17,13 +18,55 @@
 
 namespace issm {
 
-// A tile's inputs of one thread: S tokens, V channels each
-template <bool BF, int V, int S>
-struct Raw {
-  Piece<BF, V> v[S];
-  __device__ __forceinline__ void load(const void* base, long bs, long ls, int b, int t0, int c0, int last) {
+// A thread's rows of one tensor in a tile: S tokens, V channels each.
+// BUF: behind a buffer that ends with the tile's rows (those past the end of the sequence read zero and are not stored): a row is one 32-bit
+// addition.  It takes rows that start at whole dwords and lie within 2^31 bytes of a tile; the others have 64-bit addresses, clamped to the last token.
+template <bool BF, int V, int S, bool BUF>
+struct Rows {
+  static constexpr int SIZE = BF ? 2 : 4, T = GS_TT * S;
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  __amdgpu_buffer_rsrc_t buf;
+  unsigned off, step;
+  char* base;
+  long ls;
+  int t0, end;
+  // tile k of a sequence of L tokens, the thread's first row t0
+  __device__ __forceinline__ Rows(const void* q, long bs, long ls_, int b, int k, int L, int C, int t0_, int c0) {
+    if constexpr (BUF) {
+      const int rows = min(T, L - k * T), j = t0_ - k * T;
+      const unsigned gap = (unsigned)(ls_ < 0 ? -ls_ : ls_);
+      buf = __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(q) + (b * bs + (k * (long)T + (ls_ < 0 ? rows - 1 : 0)) * ls_) * SIZE, 0,
+                                              ((rows - 1) * gap + C) * SIZE, 0x00027000);
+      off = ((unsigned)(ls_ < 0 ? rows - 1 - j : j) * gap + c0) * SIZE;
+      step = (unsigned)ls_ * SIZE;
+    } else {
+      base = (char*)const_cast<void*>(q) + (b * bs + c0) * SIZE;
+      ls = ls_ * SIZE;
+      t0 = t0_;
+      end = L - 1;
+    }
+  }
+  __device__ __forceinline__ void load(Piece<BF, V> (&v)[S]) const {
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s].load(base, b * bs + (long)min(t0 + s, last) * ls + c0);   // (behind the end: the last token again)
+    for (int s = 0; s < S; ++s) {
+      if constexpr (!BUF) v[s].load(base + min(t0 + s, end) * ls, 0);
+      else if constexpr (BF) v[s].m = __builtin_bit_cast(Half<V>, (u2)__builtin_amdgcn_raw_buffer_load_b64(buf, off + s * step, 0, 0));
+      else v[s].m = __builtin_bit_cast(Word<V>, (u4)__builtin_amdgcn_raw_buffer_load_b128(buf, off + s * step, 0, 0));
+    }
+  }
+  __device__ __forceinline__ void store(int s, const float (&f)[V]) const {
+    if constexpr (BUF) {
+      if constexpr (BF) {
+        Half<V> m;
+        m.put(f);
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, m), buf, off + s * step, 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), buf, off + s * step, 0, 0);
+      }
+    } else if (t0 + s <= end) {
+      Piece<BF, V>::store(base + (t0 + s) * ls, 0, f);
+    }
   }
 };
 
@@ -69,294 +112,440 @@ __device__ __forceinline__ void tile_starts(const float (&sP)[TT][W], float (&sH
   }
 }
 
+template <int TT, int W>
+__device__ __forceinline__ void column_sum(const float (&s)[TT][W], int w, float* to) {
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int j = 0; j < TT; ++j) sum += s[j][w];
+  *to = sum;
+}
+// A thread's rows of A; whether no decay of the wave's leaves the series
+template <int V>
+__device__ __forceinline__ bool decays(const float* from, float (&A)[V]) {
+  bool near = true;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    A[v] = from[v];
+    near = near && fabsf(A[v]) < GS_NEAR;
+  }
+  return __all(near);
+}
+
 // The state in front of the o-th tile of a row (in the order of the walk), a channel a lane, from what the tiles in front of it have told:
 // the nearest state among the last GS_LOOK of them, and the maps from there on, in the order in which the tiles themselves apply
 // them -- whichever of the states is found, the bits are the same.
 // Every wait ends: tiles are taken in their order (tickets), so the tiles in front of this one are on workgroups that run, and the first of them
 // that has not told its state waits for none that has not.  (After GS_POLLS looks, seconds, it would end with NaN: should memory be overwritten
 // from elsewhere, no workgroup stays.)
-constexpr int GS_LOOK = 8, GS_POLLS = 1 << 22;
-__device__ __forceinline__ float look_back(const unsigned long long* words, int o, float first, int lane) {
-  float H[GS_LOOK], P[GS_LOOK];
-  int n = GS_LOOK;
-  for (int polls = 0; polls < GS_POLLS; ++polls) {
-    unsigned long long w[GS_LOOK];
+constexpr int GS_POLLS = 1 << 22;
+struct Look {
+  unsigned H[GS_LOOK], P[GS_LOOK];
+  __device__ __forceinline__ void ask(const unsigned long long* at) {   // at: the lane's word of the tile
 #pragma unroll
-    for (int i = 0; i < GS_LOOK; ++i)
-      w[i] = __hip_atomic_load(words + (long)max(o - 1 - i, 0) * 64 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    n = GS_LOOK;
-    bool told = true;
-#pragma unroll
-    for (int i = 0; i < GS_LOOK; ++i) {
-      unsigned high = (unsigned)(w[i] >> 32);
-      H[i] = __uint_as_float((unsigned)w[i]);
-      if (o - 1 - i < 0) {   // in front of the first: the state that the row starts from
-        high = GS_STATE;
-        H[i] = first;
-      }
-      P[i] = __uint_as_float(high);
-      if (told && n == GS_LOOK && high == GS_STATE) n = i;
-      told = told && high != GS_NOTHING;
+    for (int i = 0; i < GS_LOOK; ++i) {   // (in front of a row's first tile lie GS_LOOK that tell nothing)
+      const unsigned long long w = __hip_atomic_load(at - 64 * (i + 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      P[i] = (unsigned)(w >> 32);
+      H[i] = (unsigned)w;
     }
-    if (__all(n < GS_LOOK)) break;
-    __builtin_amdgcn_s_sleep(2);
   }
-  float h = __builtin_nanf("");
+  // (the first look asked for before)
+  __device__ __forceinline__ float back(const unsigned long long* at, int o, float first) {
+    int n = GS_LOOK;
+    for (int polls = 0;;) {
+      n = GS_LOOK;
+      bool told = true;
 #pragma unroll
-  for (int i = GS_LOOK - 1; i >= 0; --i) h = i == n ? H[i] : i < n ? fmaf(P[i], h, H[i]) : h;
-  return h;
-}
-// The tile's ticket; one barrier
-__device__ __forceinline__ int ticket(unsigned* counter, int* shared) {
-  if (threadIdx.x == 0) *shared = (int)(__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u);
-  __syncthreads();
-  return *shared;
+      for (int i = 0; i < GS_LOOK; ++i) {   // i == o: the state that the row starts from
+        if (told && n == GS_LOOK && (i == o || P[i] == GS_STATE)) n = i;
+        told = told && P[i] != GS_NOTHING;
+      }
+      if (__all(n < GS_LOOK) || ++polls == GS_POLLS) break;
+      __builtin_amdgcn_s_sleep(1);
+      ask(at);
+    }
+    float h = __builtin_nanf("");
+#pragma unroll
+    for (int i = GS_LOOK - 1; i >= 0; --i) {
+      const float f = __uint_as_float(H[i]);
+      h = i == n ? (i == o ? first : f) : i < n ? fmaf(__uint_as_float(P[i]), h, f) : h;
+    }
+    return h;
+  }
+};
+// (its answer is one less than the ticket: the counter starts with all bits set)
+__device__ __forceinline__ int ticket(unsigned* counter) {
+  return (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __global__ __launch_bounds__(256) void k_gscan_clear(uint4* p, long n) {
   for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
-// LOOK: a tile a workgroup; else a row's tiles one behind the other on one
-template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ, bool LOOK>
-__global__ __launch_bounds__(GS_THREADS) void k_gscan_fwd(GScanP p) {
-  constexpr int TT = GS_TT, W = GS_CG * V, T = TT * S;
-  __shared__ float sP[TT][W], sH[TT][W];
-  const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG;
-  const int chain = LOOK ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
-  const int c0 = first_channel<V>(cb * W + cg * V, p.C), mine = slot_channel<V>(cb * W, tid, p.C);
-  float A[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) A[v] = p.A[c0 + v];
-  float carry = 0.0f;
-  if (tid < W && p.h0) carry = p.h0[(long)b * p.C + mine];
-  __shared__ int turn;
-  const int k0 = LOOK ? ticket(p.tickets + (long)chain * GS_TICKET, &turn) : 0, k1 = LOOK ? k0 + 1 : p.nk;
-  unsigned long long* words = p.words + (long)chain * p.nk * 64;
-  for (int k = k0; k < k1; ++k) {
-    const int t0 = k * T + tt * S;
-    Raw<BF, V, S> x, g, in;
-    x.load(p.x, p.xb, p.xl, b, t0, c0, p.L - 1);
-    g.load(p.g, p.gb, p.gl, b, t0, c0, p.L - 1);
-    if (IG) in.load(p.i, p.ib, p.il, b, t0, c0, p.L - 1);
-    const unsigned cut = SEQ ? cuts<S>(p, b, t0) : 0u;
-    float a[S][V], f[S][V], P[V], H[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      P[v] = 1.0f;
-      H[v] = 0.0f;
+// A row of a block of channels is one workgroup's, tile behind tile, or (SHARED) that of several: each takes the next tile that none has taken.
+// One barrier a tile.  From a tile's barrier to the next one's the maps' wave has its maps, looks for the state in front of it and gives the
+// threads theirs; meanwhile the others ask for the inputs of the tile behind it, finish the one before it, whose states lie there, and leave
+// the maps of the one behind it.  So a state in front of a tile may be late by all of that before it costs time.
+template <int W>
+struct Maps {
+  float P[GS_TT][W], H[GS_TT][W];
+};
+template <int W>
+struct FwdShared {
+  Maps<W> maps[2];   // of two tiles in turn
+  int turn[2];       // the tile behind them
+};
+// Forward, the maps' wave
+template <int V, int S, bool SEQ, bool SHARED, int W>
+__device__ __forceinline__ void chain_fwd(const GScanP& p, FwdShared<W>& sh, int chain, int cb, int b, int k) {
+  const int w = threadIdx.x & 63, mine = slot_channel<V>(cb * W, w, p.C);
+  const bool on = W == 64 || w < W;
+  unsigned long long* words = p.words + ((long)chain * (p.nk + GS_LOOK) + GS_LOOK) * 64 + w;
+  unsigned* counter = p.tickets + (long)chain * GS_TICKET;
+  const float first = on && p.h0 ? p.h0[(long)b * p.C + mine] : 0.0f;
+  float carry = first;
+  __builtin_amdgcn_s_setprio(3);
+  for (int n = 0; k < p.nk; n ^= 1) {
+    int next = k + 1;
+    if (SHARED) {
+      if (w == 0) sh.turn[n] = ticket(counter) + 1;
+      next = __builtin_amdgcn_readfirstlane(sh.turn[n]);
     }
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float u = x.v[s][v];
-        if (IG) u *= sigmoid(in.v[s][v]);
-        float beta;
-        decay<NRM>(A[v] * sigmoid(g.v[s][v]), a[s][v], beta);
-        f[s][v] = NRM ? beta * u : u;
-      }
-    if (t0 + S > p.L) {   // behind the end: the identity
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (t0 + s >= p.L)
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            a[s][v] = 1.0f;
-            f[s][v] = 0.0f;
-          }
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const bool z = SEQ && (cut >> s & 1);
-        H[v] = z ? f[s][v] : fmaf(a[s][v], H[v], f[s][v]);
-        P[v] = z || (SEQ && P[v] < 0.0f) ? -1.0f : P[v] * a[s][v];
-      }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sP[tt][cg * V + v] = P[v];
-      sH[tt][cg * V + v] = H[v];
-    }
+    Look look;
+    if (SHARED && k > 0) look.ask(words + (long)k * 64);
     __syncthreads();
-    if (tid < W) {
+    Maps<W>& m = sh.maps[n];
+    if (on) {
       float Pt, Ht;
-      tile_map<SEQ, TT, W>(sP, sH, tid, false, Pt, Ht);
-      if (LOOK && k > 0) {
-        const bool cut_off = SEQ && Pt < 0.0f;
-        tell(words + (long)k * 64 + tid, Ht, cut_off ? GS_STATE : map_bits(Pt));
-        carry = look_back(words, k, carry, tid);
+      tile_map<SEQ, GS_TT, W>(m.P, m.H, w, false, Pt, Ht);
+      const bool cut_off = SEQ && Pt < 0.0f;
+      if (SHARED && k > 0) {
+        tell(words + (long)k * 64, Ht, cut_off ? GS_STATE : map_bits(Pt));
+        carry = look.back(words + (long)k * 64, k, first);
       }
-      if (p.hs) p.hs[((long)b * p.nk + k) * p.C + mine] = carry;
-      const float behind = SEQ && Pt < 0.0f ? Ht : fmaf(Pt, carry, Ht);
-      if (LOOK && k + 1 < p.nk) tell(words + (long)k * 64 + tid, behind, GS_STATE);
-      tile_starts<SEQ, TT, W>(sP, sH, tid, false, carry);
+      const float behind = cut_off ? Ht : fmaf(Pt, carry, Ht);
+      if (SHARED && k + 1 < p.nk) tell(words + (long)k * 64, behind, GS_STATE);
+      tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, carry);
+      if (p.hs)
+#pragma unroll
+        for (int i = 0; i < S / GS_S_BACK; ++i) {
+          const int t = k * (S / GS_S_BACK) + i;
+          if (t < p.nb) p.hs[((long)b * p.nb + t) * p.C + mine] = m.H[i * (GS_TT * GS_S_BACK / S)][w];
+        }
       carry = behind;
     }
+    k = next;
+  }
+  __syncthreads();
+}
+// IG, NRM: whether there is an in_gate, a beta; 2: asked when run.
+template <bool BF, int V, int S, int IG, int NRM, bool SEQ, bool SHARED, bool BUF>
+__global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) {
+  constexpr int W = GS_CG * V, T = GS_TT * S;
+  __shared__ FwdShared<W> sh;
+  const int chain = SHARED ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
+  const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int k = 0;
+  if (SHARED) {
+    if (tid == 0) sh.turn[1] = ticket(p.tickets + (long)chain * GS_TICKET) + 1;
     __syncthreads();
+    k = __builtin_amdgcn_readfirstlane(sh.turn[1]);   // (turn[1] is written again behind the first tile's barrier)
+  }
+  if (wave == GS_THREADS / 64 - 1) return chain_fwd<V, S, SEQ, SHARED, W>(p, sh, chain, cb, b, k);
+  const bool ig = IG == 2 ? p.i != nullptr : IG == 1, nrm = NRM == 2 ? p.nrm : NRM == 1;
+  const int c0 = first_channel<V>(cb * W + cg * V, p.C);
+  float A[V];
+  const bool all_near = decays<V>(p.A + c0, A);
+  Piece<BF, V> x[S], g[S], in[S];
+  auto request = [&](int k) {
+    const int t0 = k * T + tt * S;
+    Rows<BF, V, S, BUF>(p.x, p.xb, p.xl, b, k, p.L, p.C, t0, c0).load(x);
+    Rows<BF, V, S, BUF>(p.g, p.gb, p.gl, b, k, p.L, p.C, t0, c0).load(g);
+    if (ig) Rows<BF, V, S, BUF>(p.i, p.ib, p.il, b, k, p.L, p.C, t0, c0).load(in);
+  };
+  struct Tile {   // of a tile whose states are looked for
+    float a[S][V], f[S][V];
+    unsigned cut;
+    int k;
+  };
+  auto begin = [&](Tile& q, int k, Maps<W>& m) {
+    const int t0 = k * T + tt * S;
+    q.k = k;
+    q.cut = SEQ ? cuts<S>(p, b, t0) : 0u;
+    auto gates = [&](auto near) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (V > 1) {
+          x[s].template apart<near.value>();
+          g[s].template apart<near.value>();
+          if (ig) in[s].template apart<near.value>();
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float u = x[s][v], beta;
+          if (ig) u *= sigmoid(in[s][v]);
+          decay<near.value>(A[v] * sigmoid(g[s][v]), nrm, q.a[s][v], beta);
+          q.f[s][v] = nrm ? beta * u : u;
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (a token's values at a time are enough to fill the pipeline, and all at once cost registers)
+      }
+    };
+    if (all_near) gates(std::true_type());
+    else gates(std::false_type());
+    if ((k + 1) * T > p.L) {   // behind the end: the identity
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const bool there = t0 + s < p.L;
+          q.a[s][v] = there ? q.a[s][v] : 1.0f;
+          q.f[s][v] = there ? q.f[s][v] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float P = 1.0f, H = 0.0f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const bool z = SEQ && (q.cut >> s & 1);
+        H = z ? q.f[s][v] : fmaf(q.a[s][v], H, q.f[s][v]);
+        P = z || (SEQ && P < 0.0f) ? -1.0f : P * q.a[s][v];
+      }
+      m.P[tt][cg * V + v] = P;
+      m.H[tt][cg * V + v] = H;
+    }
+  };
+  auto finish = [&](const Tile& q, const Maps<W>& m) {
+    const int t0 = q.k * T + tt * S;
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = sH[tt][cg * V + v];
+    for (int v = 0; v < V; ++v) h[v] = m.H[tt][cg * V + v];
+    const Rows<BF, V, S, BUF> y(p.y, p.yb, p.yl, b, q.k, p.L, p.C, t0, c0);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = SEQ && (cut >> s & 1) ? f[s][v] : fmaf(a[s][v], h[v], f[s][v]);
-      const int t = t0 + s;
-      if (t < p.L) Piece<BF, V>::store(p.y, b * p.yb + t * p.yl + c0, h);
-      if (t == p.L - 1 && p.last) Piece<false, V>::store(p.last, (long)b * p.C + c0, h);
+      for (int v = 0; v < V; ++v) h[v] = SEQ && (q.cut >> s & 1) ? q.f[s][v] : fmaf(q.a[s][v], h[v], q.f[s][v]);
+      y.store(s, h);
+      if (t0 + s == p.L - 1 && p.last) Piece<false, V>::store(p.last, (long)b * p.C + c0, h);
     }
-    if (!LOOK) __syncthreads();   // (the next tile's maps go where these states are read)
+  };
+  Tile one, two;
+  one.k = two.k = -1;
+  if (k < p.nk) request(k);
+  // (a thread reads and writes no slots of the maps but its own: those of the tile that it finishes take the next one's)
+  while (k < p.nk) {
+    begin(one, k, sh.maps[0]);
+    __syncthreads();
+    k = SHARED ? __builtin_amdgcn_readfirstlane(sh.turn[0]) : k + 1;
+    if (k < p.nk) request(k);
+    if (two.k >= 0) finish(two, sh.maps[1]);
+    two.k = -1;
+    if (k >= p.nk) break;
+    begin(two, k, sh.maps[1]);
+    __syncthreads();
+    k = SHARED ? __builtin_amdgcn_readfirstlane(sh.turn[1]) : k + 1;
+    if (k < p.nk) request(k);
+    finish(one, sh.maps[0]);
+    one.k = -1;
   }
+  __syncthreads();
+  if (one.k >= 0) finish(one, sh.maps[0]);
+  if (two.k >= 0) finish(two, sh.maps[1]);
 }
 
-template <bool BF, int V, int S, bool IG, bool NRM, bool SEQ, bool LOOK>
-__global__ __launch_bounds__(GS_THREADS) void k_gscan_bwd(GScanP p) {
-  constexpr int TT = GS_TT, W = GS_CG * V, T = TT * S;
-  __shared__ float sP[TT][W], sH[TT][W], sC[TT][W];
-  const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG;
-  const int chain = LOOK ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
-  const int c0 = first_channel<V>(cb * W + cg * V, p.C), mine = slot_channel<V>(cb * W, tid, p.C);
-  float A[V], dA[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    A[v] = p.A[c0 + v];
-    dA[v] = 0.0f;
-  }
-  float carry = 0.0f;   // what the tokens behind the tile give to its last state
-  if (tid < W && p.dlast) carry = p.dlast[(long)b * p.C + mine];
-  __shared__ int turn;
-  const int o0 = LOOK ? ticket(p.tickets + (long)chain * GS_TICKET, &turn) : 0, o1 = LOOK ? o0 + 1 : p.nk;
-  unsigned long long* words = p.words + (long)chain * p.nk * 64;
-  for (int o = o0; o < o1; ++o) {   // from the last tile to the first
-    const int k = p.nk - 1 - o;
-    const int t0 = k * T + tt * S;
-    Raw<BF, V, S> x, g, in, dy;
-    x.load(p.x, p.xb, p.xl, b, t0, c0, p.L - 1);
-    g.load(p.g, p.gb, p.gl, b, t0, c0, p.L - 1);
-    if (IG) in.load(p.i, p.ib, p.il, b, t0, c0, p.L - 1);
-    if (p.dy) dy.load(p.dy, p.dyb, p.dyl, b, t0, c0, p.L - 1);
-    const unsigned cut = SEQ ? cuts<S>(p, b, t0) : 0u;
-    float a[S][V], f[S][V], d[S][V], P[V], H[V], Cm[V];
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float u = x.v[s][v];
-        if (IG) u *= sigmoid(in.v[s][v]);
-        float beta;
-        decay<NRM>(A[v] * sigmoid(g.v[s][v]), a[s][v], beta);
-        f[s][v] = NRM ? beta * u : u;
-        d[s][v] = p.dy ? dy.v[s][v] : 0.0f;
-      }
-    if (t0 + S > p.L) {
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (t0 + s >= p.L)
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            a[s][v] = 1.0f;
-            f[s][v] = d[s][v] = 0.0f;
-          }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      P[v] = 1.0f;
-      H[v] = Cm[v] = 0.0f;
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const bool z = SEQ && (cut >> s & 1);
-        H[v] = z ? f[s][v] : fmaf(a[s][v], H[v], f[s][v]);
-        P[v] = z || (SEQ && P[v] < 0.0f) ? -1.0f : P[v] * a[s][v];
-      }
-#pragma unroll
-    for (int s = S - 1; s >= 0; --s)
-#pragma unroll
-      for (int v = 0; v < V; ++v) Cm[v] = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * (d[s][v] + Cm[v]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sP[tt][cg * V + v] = P[v];
-      sH[tt][cg * V + v] = H[v];
-      sC[tt][cg * V + v] = Cm[v];
-    }
+// Backwards the tiles' order o is from the last to the first.  The maps' wave: c, what the tokens behind a tile give to its last state, and h
+// (two barriers a tile: what the threads keep of a tile is too much to keep two of, and three workgroups a CU stand in for each other)
+template <int W>
+struct BackMaps : Maps<W> {
+  int turn;
+  float C[GS_TT][W];
+  float dA[2][GS_TT][W];   // what the threads give to dA, of two tiles in turn
+};
+template <int V, int S, bool SEQ, bool SHARED, int W>
+__device__ __forceinline__ void chain_bwd(const GScanP& p, BackMaps<W>& m, int chain, int cb, int b, int o) {
+  const int w = threadIdx.x & 63, mine = slot_channel<V>(cb * W, w, p.C);
+  const bool on = W == 64 || w < W;
+  unsigned long long* words = p.words + ((long)chain * (p.nk + GS_LOOK) + GS_LOOK) * 64 + w;
+  unsigned* counter = p.tickets + (long)chain * GS_TICKET;
+  const float first = on && p.dlast ? p.dlast[(long)b * p.C + mine] : 0.0f;
+  float carry = first;
+  int past = -1, n = 0;   // the tile before this one, how many tiles
+  // a tile's sum to a row of its own: which workgroup took it is chance
+  auto sum_up = [&] {
+    if (SHARED && p.part && on && past >= 0) column_sum(m.dA[(n & 1) ^ 1], w, p.part + ((long)b * p.nk + p.nk - 1 - past) * p.C + mine);
+  };
+  __builtin_amdgcn_s_setprio(3);
+  while (o < p.nk) {
+    int next = o;
+    if (SHARED && w == 0) next = ticket(counter);
+    const float before = on ? p.hs[((long)b * p.nk + p.nk - 1 - o) * p.C + mine] : 0.0f;
+    Look look;
+    if (SHARED && o > 0) look.ask(words + (long)o * 64);
+    if (SHARED && w == 0) m.turn = next + 1;
     __syncthreads();
-    if (tid < W) {
+    next = SHARED ? __builtin_amdgcn_readfirstlane(m.turn) : o + 1;
+    if (on) {
       float Pt, Ct;
-      const float before = p.hs[((long)b * p.nk + k) * p.C + mine];
-      tile_map<SEQ, TT, W>(sP, sC, tid, true, Pt, Ct);
-      if (LOOK && o > 0) {
-        tell(words + (long)o * 64 + tid, Ct, SEQ && Pt < 0.0f ? GS_STATE : map_bits(Pt));
-        carry = look_back(words, o, carry, tid);
+      tile_map<SEQ, GS_TT, W>(m.P, m.C, w, true, Pt, Ct);
+      const bool cut_off = SEQ && Pt < 0.0f;
+      if (SHARED && o > 0) {
+        tell(words + (long)o * 64, Ct, cut_off ? GS_STATE : map_bits(Pt));
+        carry = look.back(words + (long)o * 64, o, first);
       }
-      const float behind = SEQ && Pt < 0.0f ? Ct : fmaf(Pt, carry, Ct);
-      if (LOOK && o + 1 < p.nk) tell(words + (long)o * 64 + tid, behind, GS_STATE);
-      tile_starts<SEQ, TT, W>(sP, sC, tid, true, carry);
-      tile_starts<SEQ, TT, W>(sP, sH, tid, false, before);
+      const float behind = cut_off ? Ct : fmaf(Pt, carry, Ct);
+      if (SHARED && o + 1 < p.nk) tell(words + (long)o * 64, behind, GS_STATE);
+      tile_starts<SEQ, GS_TT, W>(m.P, m.C, w, true, carry);
+      tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, before);
       carry = behind;
     }
     __syncthreads();
-    float h[V], c[V];
+    sum_up();
+    past = o;
+    ++n;
+    o = next;
+  }
+  __syncthreads();
+  sum_up();
+}
+template <bool BF, int V, int S, int IG, int NRM, bool SEQ, bool SHARED, bool BUF>
+__global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(GScanP p) {
+  constexpr int W = GS_CG * V, T = GS_TT * S;
+  __shared__ BackMaps<W> m;
+  const int chain = SHARED ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
+  const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int k0 = 0;
+  if (SHARED) {
+    if (tid == 0) m.turn = ticket(p.tickets + (long)chain * GS_TICKET) + 1;
+    __syncthreads();
+    k0 = __builtin_amdgcn_readfirstlane(m.turn);
+    __syncthreads();
+  }
+  float dA[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = sH[tt][cg * V + v];
-      c[v] = sC[tt][cg * V + v];
-    }
+  for (int v = 0; v < V; ++v) dA[v] = 0.0f;
+  const int c0 = first_channel<V>(cb * W + cg * V, p.C);
+  if (wave == GS_THREADS / 64 - 1) {
+    chain_bwd<V, S, SEQ, SHARED, W>(p, m, chain, cb, b, k0);
+  } else {
+    const bool ig = IG == 2 ? p.i != nullptr : IG == 1, nrm = NRM == 2 ? p.nrm : NRM == 1;
+    float A[V];
+    const bool all_near = decays<V>(p.A + c0, A);
+    int o = k0, n = 0;
+    while (o < p.nk) {
+      const int k = p.nk - 1 - o, t0 = k * T + tt * S;
+      Piece<BF, V> x[S], g[S], in[S], dy[S];
+      Rows<BF, V, S, BUF>(p.x, p.xb, p.xl, b, k, p.L, p.C, t0, c0).load(x);
+      Rows<BF, V, S, BUF>(p.g, p.gb, p.gl, b, k, p.L, p.C, t0, c0).load(g);
+      if (ig) Rows<BF, V, S, BUF>(p.i, p.ib, p.il, b, k, p.L, p.C, t0, c0).load(in);
+      if (p.dy) Rows<BF, V, S, BUF>(p.dy, p.dyb, p.dyl, b, k, p.L, p.C, t0, c0).load(dy);
+      const unsigned cut = SEQ ? cuts<S>(p, b, t0) : 0u;
+      float a[S][V], r[S][V], beta[S][V], sg[S][V];
+      auto gates = [&](auto near) {
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+        for (int s = 0; s < S; ++s) {
+          if (V > 1) {
+            g[s].template apart<near.value>();
+            if (ig) in[s].template apart<near.value>();
+          }
 #pragma unroll
-      for (int v = 0; v < V; ++v) {   // f becomes the state before the token
-        const bool z = SEQ && (cut >> s & 1);
-        const float now = z ? f[s][v] : fmaf(a[s][v], h[v], f[s][v]);
-        f[s][v] = z ? 0.0f : h[v];
-        h[v] = now;
+          for (int v = 0; v < V; ++v) {
+            sg[s][v] = ig ? sigmoid(in[s][v]) : 1.0f;
+            r[s][v] = sigmoid(g[s][v]);
+            decay<near.value>(A[v] * r[s][v], nrm, a[s][v], beta[s][v]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      if (all_near) gates(std::true_type());
+      else gates(std::false_type());
+      if ((k + 1) * T > p.L) {   // behind the end: the identity, and nothing to any sum
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const bool there = t0 + s < p.L;
+            a[s][v] = there ? a[s][v] : 1.0f;
+            r[s][v] = there ? r[s][v] : 0.0f;
+            sg[s][v] = there ? sg[s][v] : 0.0f;
+            beta[s][v] = there ? beta[s][v] : 0.0f;
+          }
       }
-#pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
-      float dx[V], dg[V], di[V];
+      auto d = [&](int s, int v) { return p.dy && t0 + s < p.L ? dy[s][v] : 0.0f; };
+      auto fed = [&](int s, int v) {   // the forward's beta u, rounded as there
+        const float u = ig ? x[s][v] * sg[s][v] : x[s][v];
+        return nrm ? beta[s][v] * u : t0 + s < p.L ? u : 0.0f;
+      };
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float G = d[s][v] + c[v];
-        c[v] = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * G;
-        float r, rr, sg = 1.0f, ss = 0.0f, av, beta;
-        sigmoid2(g.v[s][v], r, rr);
-        if (IG) sigmoid2(in.v[s][v], sg, ss);
-        const float l = A[v] * r, xv = x.v[s][v];
-        decay<NRM>(l, av, beta);
-        float dl = c[v] * f[s][v], du = G;
-        if (NRM) {
-          // (where nothing decays, beta = 0, the quotient's limit times l is 0)
-          dl = fmaf(-(G * (xv * sg)) * (av * av), beta == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(beta), dl);
-          du *= beta;
-        }
-        dx[v] = du * sg;
-        di[v] = du * xv * sg * ss;
-        dg[v] = dl * l * rr;
-        if (t0 + s < p.L) dA[v] = fmaf(dl, r, dA[v]);
-      }
-      const int t = t0 + s;
-      if (t < p.L) {
-        const long o = b * p.yb + t * p.yl + c0;
-        if (p.dx) Piece<BF, V>::store(p.dx, o, dx);
-        if (p.dg) Piece<BF, V>::store(p.dg, o, dg);
-        if (IG && p.di) Piece<BF, V>::store(p.di, o, di);
-      }
-      if (t == 0 && p.dh0) Piece<false, V>::store(p.dh0, (long)b * p.C + c0, c);
-    }
-    if (!LOOK) __syncthreads();
-  }
-  if (!p.part) return;
-  if (LOOK) __syncthreads();
+        float P = 1.0f, H = 0.0f, C = 0.0f;
 #pragma unroll
-  for (int v = 0; v < V; ++v) sP[tt][cg * V + v] = dA[v];
-  __syncthreads();
-  if (tid < W) {
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int j = 0; j < TT; ++j) sum += sP[j][tid];
-    p.part[((long)b * (LOOK ? p.nk : 1) + (LOOK ? p.nk - 1 - o0 : 0)) * p.C + mine] = sum;
+        for (int s = 0; s < S; ++s) {
+          const bool z = SEQ && (cut >> s & 1);
+          H = z ? fed(s, v) : fmaf(a[s][v], H, fed(s, v));
+          P = z || (SEQ && P < 0.0f) ? -1.0f : P * a[s][v];
+        }
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) C = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * (d(s, v) + C);
+        m.P[tt][cg * V + v] = P;
+        m.H[tt][cg * V + v] = H;
+        m.C[tt][cg * V + v] = C;
+      }
+      __syncthreads();
+      const int next = SHARED ? __builtin_amdgcn_readfirstlane(m.turn) : o + 1;
+      __syncthreads();
+      // (from here to the next barrier a thread reads and writes no slots of the maps but its own)
+      float h[V], c[V], before[S][V], sum[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        h[v] = m.H[tt][cg * V + v];
+        c[v] = m.C[tt][cg * V + v];
+        sum[v] = 0.0f;
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const bool z = SEQ && (cut >> s & 1);
+          before[s][v] = z ? 0.0f : h[v];
+          h[v] = z ? fed(s, v) : fmaf(a[s][v], h[v], fed(s, v));
+        }
+      const Rows<BF, V, S, BUF> to_x(p.dx, p.yb, p.yl, b, k, p.L, p.C, t0, c0), to_g(p.dg, p.yb, p.yl, b, k, p.L, p.C, t0, c0),
+          to_i(p.di, p.yb, p.yl, b, k, p.L, p.C, t0, c0);
+#pragma unroll
+      for (int s = S - 1; s >= 0; --s) {
+        float dx[V], dg[V], di[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float G = d(s, v) + c[v], l = A[v] * r[s][v], xv = x[s][v];
+          c[v] = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * G;
+          float dl = c[v] * before[s][v], du = G;
+          if (nrm) {
+            const float bt = beta[s][v];   // (0 where nothing decays: its part is left out)
+            dl = fmaf(-(G * (xv * sg[s][v])) * (a[s][v] * a[s][v]), bt == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(bt), dl);
+            du *= bt;
+          }
+          dx[v] = du * sg[s][v];
+          di[v] = dx[v] * xv * (1.0f - sg[s][v]);
+          dg[v] = dl * l * (1.0f - r[s][v]);
+          sum[v] = fmaf(dl, r[s][v], sum[v]);
+        }
+        if (p.dx) to_x.store(s, dx);
+        if (p.dg) to_g.store(s, dg);
+        if (ig && p.di) to_i.store(s, di);
+        if (t0 + s == 0 && p.dh0) Piece<false, V>::store(p.dh0, (long)b * p.C + c0, c);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (SHARED) m.dA[n & 1][tt][cg * V + v] = sum[v];
+        else dA[v] += sum[v];
+      }
+      ++n;
+      o = next;
+    }
+    if (!SHARED)
+#pragma unroll
+      for (int v = 0; v < V; ++v) m.dA[0][tt][cg * V + v] = dA[v];
+    __syncthreads();
   }
+  if (!SHARED && p.part && tid < W) column_sum(m.dA[0], tid, p.part + (long)b * p.C + slot_channel<V>(cb * W, tid, p.C));
 }
 
 // dA: the sums of `rows` partial rows, in their order
@@ -365,6 +554,7 @@ __global__ __launch_bounds__(1024) void k_gscan_sum(const float* part, int rows,
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   float sum = 0.0f;
   if (c < C)
+#pragma unroll 8
     for (int r = wv; r < rows; r += 16) sum += part[(long)r * C + c];
   s[wv][lane] = sum;
   __syncthreads();
@@ -406,7 +596,7 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
       if (v < n) {
         float u = ldv(p.x, r * p.xs + c0 + v, BF), a, beta;
         if (IG) u *= sigmoid(ldv(p.i, r * p.is + c0 + v, BF));
-        decay<NRM>(A[v] * sigmoid(ldv(p.g, r * p.gs + c0 + v, BF)), a, beta);
+        decay<false>(A[v] * sigmoid(ldv(p.g, r * p.gs + c0 + v, BF)), NRM, a, beta);
         h[v] = fmaf(a, h[v], NRM ? beta * u : u);
         stv(p.y, (long)r * p.C + c0 + v, BF, h[v]);
       }
@@ -424,59 +614,73 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
     if (v < n) state[c0 + v] = h[v];
 }
 
-template <bool BF, int V, bool IG, bool NRM, bool SEQ>
-static void launch_dir(const GScanP& p, bool back, int blocks, hipStream_t st) {
-  if (back) {
-    if (p.words) k_gscan_bwd<BF, V, GS_S, IG, NRM, SEQ, true><<<blocks, GS_THREADS, 0, st>>>(p);
-    else k_gscan_bwd<BF, V, GS_S, IG, NRM, SEQ, false><<<blocks, GS_THREADS, 0, st>>>(p);
+template <bool BF, int V, int IG, int NRM, bool SEQ, bool SHARED, bool BUF>
+static void launch_one(const GScanP& p, bool back, int blocks, hipStream_t st) {
+  if (back) k_gscan_bwd<BF, V, GS_S_BACK, IG, NRM, SEQ, SHARED, BUF><<<blocks, GS_THREADS, 0, st>>>(p);
+  else k_gscan_fwd<BF, V, SHARED ? GS_S_SHARED : GS_S_WALKED, IG, NRM, SEQ, SHARED, BUF><<<blocks, GS_THREADS, 0, st>>>(p);
+}
+template <bool BF, int V, int IG, int NRM, bool SHARED, bool BUF>
+static void launch_packed(const GScanP& p, bool back, int blocks, hipStream_t st) {
+  p.ids ? launch_one<BF, V, IG, NRM, true, SHARED, BUF>(p, back, blocks, st) : launch_one<BF, V, IG, NRM, false, SHARED, BUF>(p, back, blocks, st);
+}
+template <bool BF, int IG, int NRM>
+static void launch_shared(const GScanP& p, bool back, int blocks, hipStream_t st) {
+  p.words ? launch_packed<BF, 4, IG, NRM, true, true>(p, back, blocks, st) : launch_packed<BF, 4, IG, NRM, false, true>(p, back, blocks, st);
+}
+// Rows that buffers take: whole dwords, a tile's rows (and one more) within 2^31 bytes
+static bool behind_buffers(const GScanP& p, bool bf, bool back) {
+  if (p.C < 4) return false;
+  const long most = (1L << 31) / (4 * (GS_TT * GS_S_SHARED + 1)), odd = bf ? 1 : 0;
+  auto takes = [&](const void* q, long b, long l) { return !q || (((uintptr_t)q & 3) == 0 && !((b | l) & odd) && labs(l) < most); };
+  return !(p.C & odd) && p.C < most && takes(p.x, p.xb, p.xl) && takes(p.g, p.gb, p.gl) && takes(p.i, p.ib, p.il) &&
+         (back ? takes(p.dy, p.dyb, p.dyl) && takes(p.dx, 0, 0) && takes(p.dg, 0, 0) && takes(p.di, 0, 0) : takes(p.y, 0, 0));
+}
+template <bool BF>
+static void launch_form(const GScanP& p, bool buffers, bool back, int blocks, hipStream_t st) {
+  if (!buffers) {   // (one form for both ways of taking the tiles: a workgroup that takes all of a row's finds its own states)
+    if (p.C >= 4) launch_packed<BF, 4, 2, 2, true, false>(p, back, blocks, st);
+    else launch_packed<BF, 1, 2, 2, true, false>(p, back, blocks, st);
+  } else if (p.i) {
+    p.nrm ? launch_shared<BF, 1, 1>(p, back, blocks, st) : launch_shared<BF, 1, 0>(p, back, blocks, st);
   } else {
-    if (p.words) k_gscan_fwd<BF, V, GS_S, IG, NRM, SEQ, true><<<blocks, GS_THREADS, 0, st>>>(p);
-    else k_gscan_fwd<BF, V, GS_S, IG, NRM, SEQ, false><<<blocks, GS_THREADS, 0, st>>>(p);
+    p.nrm ? launch_shared<BF, 0, 1>(p, back, blocks, st) : launch_shared<BF, 0, 0>(p, back, blocks, st);
   }
 }
-template <bool BF, int V, bool IG, bool NRM>
-static void launch_packed(const GScanP& p, bool back, int blocks, hipStream_t st) {
-  p.ids ? launch_dir<BF, V, IG, NRM, true>(p, back, blocks, st) : launch_dir<BF, V, IG, NRM, false>(p, back, blocks, st);
-}
-template <bool BF, int V>
-static void launch_form(const GScanP& p, bool nrm, bool back, int blocks, hipStream_t st) {
-  if (p.i) nrm ? launch_packed<BF, V, true, true>(p, back, blocks, st) : launch_packed<BF, V, true, false>(p, back, blocks, st);
-  else nrm ? launch_packed<BF, V, false, true>(p, back, blocks, st) : launch_packed<BF, V, false, false>(p, back, blocks, st);
-}
 
-// Whether a row's tiles go on workgroups of their own: up to where the rows of blocks of channels fill the GPU twice.  In us, forward and backward,
-// bf16: 256 of them (8 x 4096 x 2048) 140 and 366, walked 169 and 312; 512 (32 x 2048 x 1024) 143 and 371, walked 129 and 315;
-// 32 (1 x 4096 x 2048) 22.5 and 51.5, walked 139 and 254
-bool gscan_looks(int B, int L, int C) { return gscan_tiles(L) > 1 && (long)B * gscan_blocks(C) < 2 * NCU; }
-// Bytes of a call's workspace: partial sums of dA, then the tickets and what the tiles tell, in whole 16 bytes each
-static size_t part_bytes(int B, int L, int C) { return ((size_t)B * (gscan_looks(B, L, C) ? gscan_tiles(L) : 1) * C * 4 + 255) & ~(size_t)255; }
+// Workgroups that share a row of a block of channels, of `rows` in all: as many as it takes for GS_WG a CU, forward and backward; rows enough to fill
+// the GPU twice are walked.  8 x 4096 x 2048 bf16 (256 rows) 129 and 248 us, walked 162 and 322; 16 x 4096 (512 rows) 261 and 488, walked 248
+// and 417; 1 x 131072 (32 rows) 532 and 1108, walked 4900 and 8600.
+constexpr int GS_WG = 2, GS_WG_BACK = 3, GS_ROWS_WALKED = 2 * NCU;
+static int sharing(int rows, int tiles, bool back) {
+  return rows >= GS_ROWS_WALKED ? 1 : max(1, min(tiles, ((back ? GS_WG_BACK : GS_WG) * NCU + rows - 1) / rows));
+}
+// A call's workspace: partial sums of dA, then the tickets and what the tiles tell, in whole 16 bytes each; for the finest tiles it may take
+static size_t part_bytes(int B, int L, int C) { return ((size_t)B * gscan_tiles(L, GS_S_BACK) * C * 4 + 255) & ~(size_t)255; }
 static size_t ticket_bytes(int B, int C) { return (size_t)B * gscan_blocks(C) * GS_TICKET * 4; }
-static size_t word_bytes(int B, int L, int C) { return (size_t)B * gscan_blocks(C) * gscan_tiles(L) * 64 * 8; }
+static size_t word_bytes(int B, int L, int C, int S) { return (size_t)B * gscan_blocks(C) * (gscan_tiles(L, S) + GS_LOOK) * 64 * 8; }
 size_t gscan_workspace(int B, int L, int C, bool back) {
-  return (back ? part_bytes(B, L, C) : 0) + (gscan_looks(B, L, C) ? ticket_bytes(B, C) + word_bytes(B, L, C) : 0);
+  return (back ? part_bytes(B, L, C) : 0) + ticket_bytes(B, C) + word_bytes(B, L, C, back ? GS_S_BACK : GS_S_SHARED);
 }
 
-int launch_gscan(GScanP p, bool bf, bool nrm, bool back, void* workspace, hipStream_t st) {
-  const bool wide = p.C >= 4;
+int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st) {
   p.ncb = gscan_blocks(p.C);
-  p.nk = gscan_tiles(p.L);
-  int blocks = p.B * p.ncb, rows = p.B;
+  p.nb = gscan_tiles(p.L, GS_S_BACK);
+  const int rows = p.B * p.ncb, S = back ? GS_S_BACK : GS_S_SHARED, share = sharing(rows, gscan_tiles(p.L, S), back);
+  const bool buffers = behind_buffers(p, bf, back), shared = share > 1 || !buffers;
+  p.nk = shared || back ? gscan_tiles(p.L, S) : gscan_tiles(p.L, GS_S_WALKED);
   char* ws = (char*)workspace;
   if (back) {
     p.part = p.dA ? (float*)ws : nullptr;
     ws += part_bytes(p.B, p.L, p.C);
   }
-  if (gscan_looks(p.B, p.L, p.C)) {
+  if (shared) {
     p.tickets = (unsigned*)ws;
     p.words = (unsigned long long*)(ws + ticket_bytes(p.B, p.C));
-    const long n = (long)((ticket_bytes(p.B, p.C) + word_bytes(p.B, p.L, p.C)) / 16);
+    const long n = (long)((ticket_bytes(p.B, p.C) + word_bytes(p.B, p.L, p.C, S)) / 16);
     k_gscan_clear<<<(int)min((n + 1023) / 1024, 1024L), 256, 0, st>>>((uint4*)ws, n);
-    blocks *= p.nk;
-    rows *= p.nk;
   }
-  if (bf) wide ? launch_form<true, 4>(p, nrm, back, blocks, st) : launch_form<true, 1>(p, nrm, back, blocks, st);
-  else wide ? launch_form<false, 4>(p, nrm, back, blocks, st) : launch_form<false, 1>(p, nrm, back, blocks, st);
-  if (p.part) k_gscan_sum<<<(p.C + 63) / 64, 1024, 0, st>>>(p.part, rows, p.C, p.dA);
+  bf ? launch_form<true>(p, buffers, back, rows * share, st) : launch_form<false>(p, buffers, back, rows * share, st);
+  if (p.part) k_gscan_sum<<<(p.C + 63) / 64, 1024, 0, st>>>(p.part, shared ? p.B * p.nk : p.B, p.C, p.dA);
   return (int)hipGetLastError();
 }
 

@@ -4,10 +4,15 @@
 
 namespace issm {
 
-constexpr int GS_THREADS = 512, GS_CG = 16, GS_TT = GS_THREADS / GS_CG, GS_S = 4, GS_TILE = GS_TT * GS_S;   // tokens of a tile
+// A workgroup: GS_TT segments of tokens times GS_CG groups of channels, and a wave that joins the segments' maps
+constexpr int GS_THREADS = 512, GS_CG = 16, GS_TT = (GS_THREADS - 64) / GS_CG;
+// Tokens of a thread: forward, in workgroups that share a row and in ones that walk it, and backward.  The forward leaves the states in front of
+// the backward's tiles.
+constexpr int GS_S_SHARED = 4, GS_S_WALKED = 2, GS_S_BACK = 2, GS_TILE_BACK = GS_TT * GS_S_BACK;
 
 struct GScanP {
-  int B, L, C, ncb, nk;           // ncb, nk: blocks of channels, tiles of tokens
+  int B, L, C, ncb, nk, nb;       // ncb, nk, nb: blocks of channels, tiles of tokens, the backward's
+  bool nrm;
   const void *x, *g, *i, *dy;     // i, dy: or NULL
   long xb, xl, gb, gl, ib, il, dyb, dyl;   // strides of batch and token in elements; negative ones walk from the end
   const float *A, *h0, *dlast;    // (C); (B, C) or NULL
@@ -15,11 +20,11 @@ struct GScanP {
   long ids_b, ids_l;
   void *y, *dx, *dg, *di;         // yb, yl: strides of all four
   long yb, yl;
-  float *last, *hs, *dh0, *part, *dA;   // (B, C); (B, nk, C) states before the tiles; (B, C); partial sums of dA; (C)
+  float *last, *hs, *dh0, *part, *dA;   // (B, C); (B, tiles of the backward, C) states in front of them; (B, C); partial sums of dA; (C)
   unsigned* tickets;              // tiles of a row on workgroups of their own: a counter for each row of a block of channels, GS_TICKET apart, and
-  unsigned long long* words;      // what its tiles tell the ones behind them, (B, ncb, nk, 64); all bits set before the launch
+  unsigned long long* words;      // what its tiles tell the ones behind them, (B, ncb, GS_LOOK + nk, 64); all bits set before the launch
 };
-constexpr int GS_TICKET = 32;
+constexpr int GS_TICKET = 32, GS_LOOK = 4;
 
 // What a tile tells the ones behind it of a channel, in one access of 8 bytes, so that nothing needs an order of its own: the map of its tokens,
 // H below P, or the state behind it, H below the bits of -0 (P is never negative: a tile with a cut knows the state behind it), or, all bits set,
@@ -43,7 +48,7 @@ struct GStepP {
 };
 
 inline int gscan_blocks(int C) { return C >= 4 ? (C + GS_CG * 4 - 1) / (GS_CG * 4) : 1; }
-inline int gscan_tiles(int L) { return (int)(((long)L + GS_TILE - 1) / GS_TILE); }
+inline int gscan_tiles(int L, int S) { return (int)(((long)L + GS_TT * S - 1) / (GS_TT * S)); }
 
 // The first of a thread's V channels: where fewer than V are left they are the last V, and two threads compute the same values
 template <int V>
@@ -53,63 +58,76 @@ template <int V>
 __device__ __forceinline__ int slot_channel(int c, int slot, int C) { return first_channel<V>(c + slot / V * V, C) + slot % V; }
 
 // V elements side by side, at any element's address: types that promise no more than an element's alignment (the target takes
-// wide accesses at any address)
+// wide accesses at any address).  Pairs of bf16 stay one register: as halves the compiler keeps each in a register of its own.
 template <int N>
 struct __attribute__((packed, aligned(2))) Half {
-  uint16_t v[N];
+  unsigned v[N / 2];
+  __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16); }
+  __device__ __forceinline__ void put(const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
+  }
+};
+template <>
+struct Half<1> {
+  uint16_t v;
+  __device__ __forceinline__ float operator[](int) const { return bf16_to_f(v); }
+  __device__ __forceinline__ void put(const float (&f)[1]) { v = f_to_bf16(f[0]); }
 };
 template <int N>
 struct __attribute__((packed, aligned(4))) Word {
   float v[N];
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+  __device__ __forceinline__ void put(const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = f[i];
+  }
 };
 template <bool BF, int V>
 struct Piece {
   using Mem = typename std::conditional<BF, Half<V>, Word<V>>::type;
+  using Element = typename std::conditional<BF, uint16_t, float>::type;
   Mem m;
-  __device__ __forceinline__ void load(const void* p, long off) {
-    if constexpr (BF) m = *(const Mem*)((const uint16_t*)p + off);
-    else m = *(const Mem*)((const float*)p + off);
-  }
-  __device__ __forceinline__ float operator[](int v) const {
-    if constexpr (BF) return bf16_to_f(m.v[v]);
-    else return m.v[v];
+  __device__ __forceinline__ void load(const void* p, long off) { m = *(const Mem*)((const Element*)p + off); }
+  __device__ __forceinline__ float operator[](int v) const { return m[v]; }
+  // Its registers as something new to the compiler: two ways behind a branch that begin with the same conversions would have all of them in
+  // front of it, in registers of their own
+  template <bool WAY>
+  __device__ __forceinline__ void apart() {
+    unsigned(&w)[sizeof(Mem) / 4] = (unsigned(&)[sizeof(Mem) / 4])m;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(Mem) / 4; ++i) {
+      if constexpr (WAY) asm volatile("; near" : "+v"(w[i]));
+      else asm volatile("; any" : "+v"(w[i]));
+    }
   }
   static __device__ __forceinline__ void store(void* p, long off, const float (&f)[V]) {
     Mem m;
-    if constexpr (BF) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) m.v[v] = f_to_bf16(f[v]);
-      *(Mem*)((uint16_t*)p + off) = m;
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) m.v[v] = f[v];
-      *(Mem*)((float*)p + off) = m;
-    }
+    m.put(f);
+    *(Mem*)((Element*)p + off) = m;
   }
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ex2(-LOG2E * x)); }
-// and 1 - sigmoid, without its cancellation (e bounded, so that e * 0 does not arise; a NaN stays one)
-__device__ __forceinline__ void sigmoid2(float x, float& s, float& rest) {
-  float z = -LOG2E * x;
-  z = z > 126.0f ? 126.0f : z;
-  const float e = ex2(z);
-  s = __builtin_amdgcn_rcpf(1.0f + e);
-  rest = e * s;
-}
-// a = exp(l) and beta = sqrt(1 - a^2).  Near 0, -expm1(l) as its series: what is left out is below 2^-24 of it at |l| = 1/4 (l^6 / 7! = 4.8e-8)
-template <bool NRM>
-__device__ __forceinline__ void decay(float l, float& a, float& beta) {
-  const float e = ex2(LOG2E * l);
+// a = exp(l) and beta = sqrt(1 - a^2).  Up to |l| = 1/4, -expm1(l) as its series: what is left out is below 2^-24 of it (l^6 / 7! = 4.8e-8).
+// NEAR: no l is beyond that (the same values, without the other form's exponential)
+constexpr float GS_NEAR = 0.25f;
+template <bool NEAR>
+__device__ __forceinline__ void decay(float l, bool nrm, float& a, float& beta) {
   float q = fmaf(l, 1.0f / 720.0f, 1.0f / 120.0f);
   q = fmaf(l, q, 1.0f / 24.0f);
   q = fmaf(l, q, 1.0f / 6.0f);
   q = fmaf(l, q, 0.5f);
   q = fmaf(l, q, 1.0f);
-  const bool near = fabsf(l) < 0.25f;
-  const float d = near ? -l * q : 1.0f - e;
-  a = near ? 1.0f - d : e;
-  if (NRM) beta = __builtin_amdgcn_sqrtf(fmaf(d, a, d));
+  float d = -l * q;
+  a = 1.0f - d;
+  if (!NEAR) {
+    const float e = ex2(LOG2E * l);
+    const bool near = fabsf(l) < GS_NEAR;
+    d = near ? d : 1.0f - e;
+    a = near ? a : e;
+  }
+  beta = nrm ? __builtin_amdgcn_sqrtf(fmaf(d, a, d)) : 1.0f;
 }
 
 }  // namespace issm

@@ -89,7 +89,7 @@ int pgen_bwd_blocks(long tokens);
 int launch_pgen_fwd(const PGenP& p, hipStream_t st);
 int launch_pgen_bwd(const PGenP& p, hipStream_t st);
 size_t gscan_workspace(int B, int L, int C, bool back);
-int launch_gscan(GScanP p, bool bf, bool nrm, bool back, void* workspace, hipStream_t st);
+int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st);
 int launch_gscan_step(GStepP p, bool bf, bool nrm, hipStream_t st);
 int launch_rotary(RotP p, bool bf, bool inter, bool norm, hipStream_t st);
 int launch_rotary_norm_bwd(RotP p, bool bf, bool inter, hipStream_t st);
@@ -1433,7 +1433,7 @@ static int gscan_sizes(const issm_gated_scan_args* a) {
   if (!a) return fail(ISSM_E_NULL, "gated_scan: args is NULL");
   if (a->batch < 1 || a->seqlen < 1 || a->channels < 1 || a->seqlen > (1 << 30))
     return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d", a->batch, a->seqlen, a->channels);
-  if ((int64_t)a->batch * gscan_blocks(a->channels) * gscan_tiles(a->seqlen) >= (1 << 22))
+  if ((int64_t)a->batch * gscan_blocks(a->channels) * gscan_tiles(a->seqlen, 1) >= (1 << 24))
     return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d are too many tiles", a->batch, a->seqlen, a->channels);
   if (a->dtype != ISSM_F32 && a->dtype != ISSM_BF16) return fail(ISSM_E_DTYPE, "gated_scan: dtype %d", a->dtype);
   if (a->flags & ~(ISSM_GS_NORMALIZE | ISSM_GS_REVERSE)) return fail(ISSM_E_UNSUPPORTED, "gated_scan: flags 0x%x", a->flags);
@@ -1444,7 +1444,7 @@ int issm_gated_scan_saved_bytes(const issm_gated_scan_args* a, size_t* out) {
   int rc = gscan_sizes(a);
   if (rc) return rc;
   if (!out) return fail(ISSM_E_NULL, "out is NULL");
-  *out = (size_t)a->batch * gscan_tiles(a->seqlen) * a->channels * sizeof(float);
+  *out = (size_t)a->batch * gscan_tiles(a->seqlen, GS_S_BACK) * a->channels * sizeof(float);
   return ISSM_OK;
 }
 
@@ -1492,6 +1492,7 @@ static int gscan_call(const issm_gated_scan_args* a, bool back) {
   p.yb = (long)a->seqlen * a->channels;
   p.yl = reverse ? -(long)a->channels : a->channels;
   auto first = [&](void* t) { return t && reverse ? (void*)((char*)t + end * a->channels * size) : t; };
+  p.nrm = a->flags & ISSM_GS_NORMALIZE;
   p.A = a->A;
   p.h0 = a->h0;
   p.hs = (float*)a->saved;
@@ -1508,7 +1509,7 @@ static int gscan_call(const issm_gated_scan_args* a, bool back) {
   }
   if (need && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace & 15))
     return fail(ISSM_E_WORKSPACE, "gated_scan: %zu bytes of workspace, %zu needed", a->workspace_bytes, need);
-  return launched(launch_gscan(p, bf, a->flags & ISSM_GS_NORMALIZE, back, a->workspace, (hipStream_t)a->stream), back ? "gated_scan_bwd" : "gated_scan_fwd");
+  return launched(launch_gscan(p, bf, back, a->workspace, (hipStream_t)a->stream), back ? "gated_scan_bwd" : "gated_scan_fwd");
 }
 
 int issm_gated_scan_fwd(const issm_gated_scan_args* a) { return gscan_call(a, false); }
