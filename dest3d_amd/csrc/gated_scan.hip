@@ -548,70 +548,102 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
   if (!SHARED && p.part && tid < W) column_sum(m.dA[0], tid, p.part + (long)b * p.C + slot_channel<V>(cb * W, tid, p.C));
 }
 
-// dA: the sums of `rows` partial rows, in their order
+// dA: the sums of `rows` partial rows, in an order that their number alone decides: 16 channels and 64 strands of rows a workgroup
 __global__ __launch_bounds__(1024) void k_gscan_sum(const float* part, int rows, int C, float* out) {
-  __shared__ float s[16][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float sum = 0.0f;
-  if (c < C)
-#pragma unroll 8
-    for (int r = wv; r < rows; r += 16) sum += part[(long)r * C + c];
-  s[wv][lane] = sum;
+  __shared__ float s[64][17];
+  const int c = threadIdx.x & 15, strand = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
+  s[strand][c] = strand_sum(part + min(d, C - 1), C, strand, rows);
   __syncthreads();
-  if (wv || c >= C) return;
-  sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sum += s[i][lane];
-  out[c] = sum;
+  if (strand || d >= C) return;
+  float sum = 0.0f;
+#pragma unroll 16
+  for (int i = 0; i < 64; ++i) sum += s[i][c];
+  out[d] = sum;
 }
 
-// One token a row.  Rows whose slot is none of the pool's give zeros and touch no state.  Several rows of one slot are taken in their order, by
-// the first of them: a wave looks over all rows' slots, 64 at a time.
+// One token a row, four channels a thread.  Rows whose slot is none of the pool's give zeros and touch no state.  Several rows of one slot are
+// taken in their order, by the first of them: a wave looks over all rows' slots, 256 requested at a time.
+// Bound by its bytes: 512 rows of 4096 channels bf16 in a pool, 33.6 MB.
+template <bool BF>
+struct Four {   // the channels that there are of four
+  Piece<BF, 4> m;
+  __device__ __forceinline__ void load(const void* q, long off, int n) {
+    if (n >= 4) return m.load(q, off);
+    float f[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) f[v] = v < n ? ldv(q, off + v, BF) : 0.0f;
+    m.m.put(f);
+  }
+  static __device__ __forceinline__ void store(void* q, long off, int n, const float (&f)[4]) {
+    if (n >= 4) return Piece<BF, 4>::store(q, off, f);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (v < n) stv(q, off + v, BF, f[v]);
+  }
+};
 template <bool BF, bool IG, bool NRM>
 __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
   const int lane = threadIdx.x & 63, row = blockIdx.x / p.ncb;
-  const int c0 = (blockIdx.x % p.ncb * 256 + threadIdx.x) * 4, n = min(4, p.C - c0);   // (n <= 0: no channel, but votes)
+  const int c0 = (blockIdx.x % p.ncb * 256 + threadIdx.x) * 4, n = min(4, p.C - c0);   // (n <= 0: no channel, but a look at the slots)
   auto slot_of = [&](int r) { return p.at64 ? ((const long*)p.at)[r] : (long)((const int*)p.at)[r]; };
-  long slot = row;
-  if (p.at) {
-    slot = slot_of(row);
-    if (slot < 0 || slot >= p.slots) {
-      for (int v = 0; v < n; ++v) stv(p.y, (long)row * p.C + c0 + v, BF, 0.0f);
-      return;
-    }
-    bool before = false;
-    for (int r = lane; r < row; r += 64) before |= slot_of(r) == slot;
-    if (__any(before)) return;
-  }
-  float* state = p.state + slot * p.state_s;
-  float A[4], h[4];
+  Four<BF> x, g, in;
+  float A[4];
+  auto request = [&](int r) {
+    x.load(p.x, r * p.xs + c0, n);
+    g.load(p.g, r * p.gs + c0, n);
+    if (IG) in.load(p.i, r * p.is + c0, n);
+  };
+  request(row);
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    A[v] = v < n ? p.A[c0 + v] : 0.0f;
-    h[v] = v < n ? state[c0 + v] : 0.0f;
+  for (int v = 0; v < 4; ++v) A[v] = v < n ? p.A[c0 + v] : 0.0f;
+  const long slot = p.at ? slot_of(row) : row;
+  const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (slot < 0 || slot >= p.slots) return Four<BF>::store(p.y, (long)row * p.C + c0, n, none);
+  float* state = p.state + slot * p.state_s;
+  Four<false> old;
+  old.load(state, c0, n);
+  int next = p.rows;   // the next row of the slot
+  if (p.at) {
+    bool before = false;
+    for (int q = 0; q < p.rows; q += 256) {
+      long s[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = slot_of(min(q + 64 * i + lane, p.rows - 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = q + 64 * i + lane;
+        const bool same = r < p.rows && s[i] == slot;
+        before = before || (same && r < row);
+        next = same && r > row ? min(next, r) : next;
+      }
+    }
+    if (__any(before)) return;
+    if (__any(next < p.rows))
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o, 64));
   }
+  float h[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) h[v] = old.m[v];
   for (int r = row;;) {
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-      if (v < n) {
-        float u = ldv(p.x, r * p.xs + c0 + v, BF), a, beta;
-        if (IG) u *= sigmoid(ldv(p.i, r * p.is + c0 + v, BF));
-        decay<false>(A[v] * sigmoid(ldv(p.g, r * p.gs + c0 + v, BF)), NRM, a, beta);
-        h[v] = fmaf(a, h[v], NRM ? beta * u : u);
-        stv(p.y, (long)r * p.C + c0 + v, BF, h[v]);
-      }
-    if (!p.at) break;
-    int next = p.rows;   // the next row of the slot
+    for (int v = 0; v < 4; ++v) {
+      float u = x.m[v], a, beta;
+      if (IG) u *= sigmoid(in.m[v]);
+      decay<false>(A[v] * sigmoid(g.m[v]), NRM, a, beta);
+      h[v] = fmaf(a, h[v], NRM ? beta * u : u);
+    }
+    Four<BF>::store(p.y, (long)r * p.C + c0, n, h);
+    if (next >= p.rows) break;
+    r = next;
+    request(r);
+    next = p.rows;
     for (int q = r + 1; q < p.rows && next == p.rows; q += 64) {
       const unsigned long long hit = __ballot(q + lane < p.rows && slot_of(min(q + lane, p.rows - 1)) == slot);
       if (hit) next = q + __ffsll(hit) - 1;
     }
-    if (next == p.rows) break;
-    r = next;
   }
-#pragma unroll
-  for (int v = 0; v < 4; ++v)
-    if (v < n) state[c0 + v] = h[v];
+  Four<false>::store(state, c0, n, h);
 }
 
 template <bool BF, int V, int IG, int NRM, bool SEQ, bool SHARED, bool BUF>
@@ -680,7 +712,7 @@ int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st) 
     k_gscan_clear<<<(int)min((n + 1023) / 1024, 1024L), 256, 0, st>>>((uint4*)ws, n);
   }
   bf ? launch_form<true>(p, buffers, back, rows * share, st) : launch_form<false>(p, buffers, back, rows * share, st);
-  if (p.part) k_gscan_sum<<<(p.C + 63) / 64, 1024, 0, st>>>(p.part, shared ? p.B * p.nk : p.B, p.C, p.dA);
+  if (p.part) k_gscan_sum<<<(p.C + 15) / 16, 1024, 0, st>>>(p.part, shared ? p.B * p.nk : p.B, p.C, p.dA);
   return (int)hipGetLastError();
 }
 

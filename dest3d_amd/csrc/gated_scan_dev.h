@@ -130,4 +130,19 @@ __device__ __forceinline__ void decay(float l, bool nrm, float& a, float& beta) 
   beta = nrm ? __builtin_amdgcn_sqrtf(fmaf(d, a, d)) : 1.0f;
 }
 
+// The sum of rows strand, strand + 64, ... of a column, four requests at a time, in their order
+__device__ __forceinline__ float strand_sum(const float* column, int stride, int strand, int rows) {
+  float sum = 0.0f;
+  int r = strand;
+  for (; r + 192 < rows; r += 256) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = column[(long)(r + 64 * i) * stride];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += v[i];
+  }
+  for (; r < rows; r += 64) sum += column[(long)r * stride];
+  return sum;
+}
+
 }  // namespace issm
