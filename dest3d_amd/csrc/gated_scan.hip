@@ -70,20 +70,27 @@ struct Rows {
   }
 };
 
-// Which of the thread's S tokens a sequence starts at; the id before the first token is 0
+// The ids of the thread's S tokens and of the one before them, and at which of the S a sequence starts; the id before the first token is 0
 template <int S>
-__device__ __forceinline__ unsigned cuts(const GScanP& p, int b, int t0) {
-  const int* ids = p.ids + b * p.ids_b;
+struct Ids {
   int id[S + 1];
+  __device__ __forceinline__ void load(const GScanP& p, int b, int t0) {
+    const int* ids = p.ids + b * p.ids_b;
 #pragma unroll
-  for (int s = 0; s <= S; ++s) {
-    const int t = t0 + s - 1;
-    id[s] = t < 0 ? 0 : ids[(long)min(t, p.L - 1) * p.ids_l];
+    for (int s = 0; s <= S; ++s) id[s] = ids[(long)min(max(t0 + s - 1, 0), p.L - 1) * p.ids_l];
   }
-  unsigned m = 0;
+  __device__ __forceinline__ unsigned cuts(int t0) const {
+    unsigned m = (t0 ? id[0] : 0) != id[1] ? 1u : 0u;
 #pragma unroll
-  for (int s = 0; s < S; ++s) m |= id[s + 1] != id[s] ? 1u << s : 0u;
-  return m;
+    for (int s = 1; s < S; ++s) m |= id[s + 1] != id[s] ? 1u << s : 0u;
+    return m;
+  }
+};
+// What is done at each token, APART: for a wave without a cut among its tokens as in rows that are not packed
+template <bool SEQ, bool APART, class F>
+__device__ __forceinline__ void with_cuts(unsigned cut, F f) {
+  if (SEQ && (!APART || __any(cut != 0))) f([&](int s) { return (cut >> s & 1) != 0; });
+  else f([](int) { return false; });
 }
 
 // The maps of a tile's segments, as the threads leave them, a channel a lane.  P < 0 marks a segment with a cut: nothing passes through it.
@@ -252,15 +259,17 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
   if (wave == GS_THREADS / 64 - 1) return chain_fwd<V, S, SEQ, SHARED, W>(p, sh, chain, cb, b, k);
   const bool ig = IG == 2 ? p.i != nullptr : IG == 1, nrm = NRM == 2 ? p.nrm : NRM == 1;
   const int c0 = first_channel<V>(cb * W + cg * V, p.C);
-  float A[V];
-  const bool all_near = decays<V>(p.A + c0, A);
   Piece<BF, V> x[S], g[S], in[S];
+  Ids<S> ids;
   auto request = [&](int k) {
     const int t0 = k * T + tt * S;
     Rows<BF, V, S, BUF>(p.x, p.xb, p.xl, b, k, p.L, p.C, t0, c0).load(x);
     Rows<BF, V, S, BUF>(p.g, p.gb, p.gl, b, k, p.L, p.C, t0, c0).load(g);
     if (ig) Rows<BF, V, S, BUF>(p.i, p.ib, p.il, b, k, p.L, p.C, t0, c0).load(in);
+    if (SEQ) ids.load(p, b, t0);
   };
+  float A[V];
+  const bool all_near = decays<V>(p.A + c0, A);
   struct Tile {   // of a tile whose states are looked for
     float a[S][V], f[S][V];
     unsigned cut;
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
   auto begin = [&](Tile& q, int k, Maps<W>& m) {
     const int t0 = k * T + tt * S;
     q.k = k;
-    q.cut = SEQ ? cuts<S>(p, b, t0) : 0u;
+    if (SEQ) ids.load(p, b, t0);
     auto gates = [&](auto near) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -300,18 +309,20 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
           q.f[s][v] = there ? q.f[s][v] : 0.0f;
         }
     }
+    q.cut = SEQ ? ids.cuts(t0) : 0u;
+    with_cuts<SEQ, true>(q.cut, [&](auto cut) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float P = 1.0f, H = 0.0f;
+      for (int v = 0; v < V; ++v) {
+        float P = 1.0f, H = 0.0f;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const bool z = SEQ && (q.cut >> s & 1);
-        H = z ? q.f[s][v] : fmaf(q.a[s][v], H, q.f[s][v]);
-        P = z || (SEQ && P < 0.0f) ? -1.0f : P * q.a[s][v];
+        for (int s = 0; s < S; ++s) {
+          H = cut(s) ? q.f[s][v] : fmaf(q.a[s][v], H, q.f[s][v]);
+          P *= q.a[s][v];
+        }
+        m.P[tt][cg * V + v] = SEQ && q.cut ? -1.0f : P;
+        m.H[tt][cg * V + v] = H;
       }
-      m.P[tt][cg * V + v] = P;
-      m.H[tt][cg * V + v] = H;
-    }
+    });
   };
   auto finish = [&](const Tile& q, const Maps<W>& m) {
     const int t0 = q.k * T + tt * S;
@@ -319,13 +330,15 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = m.H[tt][cg * V + v];
     const Rows<BF, V, S, BUF> y(p.y, p.yb, p.yl, b, q.k, p.L, p.C, t0, c0);
+    with_cuts<SEQ, true>(q.cut, [&](auto cut) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+      for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = SEQ && (q.cut >> s & 1) ? q.f[s][v] : fmaf(q.a[s][v], h[v], q.f[s][v]);
-      y.store(s, h);
-      if (t0 + s == p.L - 1 && p.last) Piece<false, V>::store(p.last, (long)b * p.C + c0, h);
-    }
+        for (int v = 0; v < V; ++v) h[v] = cut(s) ? q.f[s][v] : fmaf(q.a[s][v], h[v], q.f[s][v]);
+        y.store(s, h);
+        if (t0 + s == p.L - 1 && p.last) Piece<false, V>::store(p.last, (long)b * p.C + c0, h);
+      }
+    });
   };
   Tile one, two;
   one.k = two.k = -1;
@@ -435,8 +448,14 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
       Rows<BF, V, S, BUF>(p.x, p.xb, p.xl, b, k, p.L, p.C, t0, c0).load(x);
       Rows<BF, V, S, BUF>(p.g, p.gb, p.gl, b, k, p.L, p.C, t0, c0).load(g);
       if (ig) Rows<BF, V, S, BUF>(p.i, p.ib, p.il, b, k, p.L, p.C, t0, c0).load(in);
-      if (p.dy) Rows<BF, V, S, BUF>(p.dy, p.dyb, p.dyl, b, k, p.L, p.C, t0, c0).load(dy);
-      const unsigned cut = SEQ ? cuts<S>(p, b, t0) : 0u;
+      if (p.dy) {
+        Rows<BF, V, S, BUF>(p.dy, p.dyb, p.dyl, b, k, p.L, p.C, t0, c0).load(dy);
+      } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s) dy[s].keep(false);
+      }
+      Ids<S> ids;
+      if (SEQ) ids.load(p, b, t0);
       float a[S][V], r[S][V], beta[S][V], sg[S][V];
       auto gates = [&](auto near) {
 #pragma unroll
@@ -458,36 +477,40 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
       else gates(std::false_type());
       if ((k + 1) * T > p.L) {   // behind the end: the identity, and nothing to any sum
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+        for (int s = 0; s < S; ++s) {
+          const bool there = t0 + s < p.L;
+          x[s].keep(there);
+          dy[s].keep(there);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const bool there = t0 + s < p.L;
             a[s][v] = there ? a[s][v] : 1.0f;
             r[s][v] = there ? r[s][v] : 0.0f;
             sg[s][v] = there ? sg[s][v] : 0.0f;
             beta[s][v] = there ? beta[s][v] : 0.0f;
           }
+        }
       }
-      auto d = [&](int s, int v) { return p.dy && t0 + s < p.L ? dy[s][v] : 0.0f; };
       auto fed = [&](int s, int v) {   // the forward's beta u, rounded as there
         const float u = ig ? x[s][v] * sg[s][v] : x[s][v];
-        return nrm ? beta[s][v] * u : t0 + s < p.L ? u : 0.0f;
+        return nrm ? beta[s][v] * u : u;
       };
+      const unsigned cuts = SEQ ? ids.cuts(t0) : 0u;
+      with_cuts<SEQ, !(BF && SHARED)>(cuts, [&](auto cut) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float P = 1.0f, H = 0.0f, C = 0.0f;
+        for (int v = 0; v < V; ++v) {
+          float P = 1.0f, H = 0.0f, C = 0.0f;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const bool z = SEQ && (cut >> s & 1);
-          H = z ? fed(s, v) : fmaf(a[s][v], H, fed(s, v));
-          P = z || (SEQ && P < 0.0f) ? -1.0f : P * a[s][v];
+          for (int s = 0; s < S; ++s) {
+            H = cut(s) ? fed(s, v) : fmaf(a[s][v], H, fed(s, v));
+            P *= a[s][v];
+          }
+#pragma unroll
+          for (int s = S - 1; s >= 0; --s) C = cut(s) ? 0.0f : a[s][v] * (dy[s][v] + C);
+          m.P[tt][cg * V + v] = SEQ && cuts ? -1.0f : P;
+          m.H[tt][cg * V + v] = H;
+          m.C[tt][cg * V + v] = C;
         }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) C = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * (d(s, v) + C);
-        m.P[tt][cg * V + v] = P;
-        m.H[tt][cg * V + v] = H;
-        m.C[tt][cg * V + v] = C;
-      }
+      });
       __syncthreads();
       const int next = SHARED ? __builtin_amdgcn_readfirstlane(m.turn) : o + 1;
       __syncthreads();
@@ -499,13 +522,13 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
         c[v] = m.C[tt][cg * V + v];
         sum[v] = 0.0f;
       }
+      with_cuts<SEQ, !(BF && SHARED)>(cuts, [&](auto cut) {
 #pragma unroll
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const bool z = SEQ && (cut >> s & 1);
-          before[s][v] = z ? 0.0f : h[v];
-          h[v] = z ? fed(s, v) : fmaf(a[s][v], h[v], fed(s, v));
+          before[s][v] = cut(s) ? 0.0f : h[v];
+          h[v] = cut(s) ? fed(s, v) : fmaf(a[s][v], h[v], fed(s, v));
         }
       const Rows<BF, V, S, BUF> to_x(p.dx, p.yb, p.yl, b, k, p.L, p.C, t0, c0), to_g(p.dg, p.yb, p.yl, b, k, p.L, p.C, t0, c0),
           to_i(p.di, p.yb, p.yl, b, k, p.L, p.C, t0, c0);
@@ -514,8 +537,8 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
         float dx[V], dg[V], di[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float G = d(s, v) + c[v], l = A[v] * r[s][v], xv = x[s][v];
-          c[v] = SEQ && (cut >> s & 1) ? 0.0f : a[s][v] * G;
+          const float G = dy[s][v] + c[v], l = A[v] * r[s][v], xv = x[s][v];
+          c[v] = cut(s) ? 0.0f : a[s][v] * G;
           float dl = c[v] * before[s][v], du = G;
           if (nrm) {
             const float bt = beta[s][v];   // (0 where nothing decays: its part is left out)
@@ -532,6 +555,7 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
         if (ig && p.di) to_i.store(s, di);
         if (t0 + s == 0 && p.dh0) Piece<false, V>::store(p.dh0, (long)b * p.C + c0, c);
       }
+      });
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (SHARED) m.dA[n & 1][tt][cg * V + v] = sum[v];

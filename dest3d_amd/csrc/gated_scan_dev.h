@@ -101,6 +101,12 @@ struct Piece {
       else asm volatile("; any" : "+v"(w[i]));
     }
   }
+  __device__ __forceinline__ void keep(bool there) {   // or zeros
+    float f[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = there ? m[v] : 0.0f;
+    m.put(f);
+  }
   static __device__ __forceinline__ void store(void* p, long off, const float (&f)[V]) {
     Mem m;
     m.put(f);

@@ -1319,11 +1319,12 @@ std::vector<Tensor> scan_layer(const Tensor& in_key, const Tensor& in_query, con
 
 // ------------------------------------------------------------------------------------------------ gated linear recurrence
 // (a tensor that is the lazy negation of its memory is computed first)
-Tensor kernel_operand(const Tensor& t, at::ScalarType type) { return t.defined() ? io_cast(t.resolve_neg(), type) : t; }
+Tensor in_memory(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor kernel_operand(const Tensor& t, at::ScalarType type) { return io_cast(in_memory(t), type); }
+// whether a call is a node's: to be differentiated, or (as the nodes say by an error) carrying a forward derivative that would be lost
 bool recorded(std::initializer_list<const Tensor*> inputs) {
-  if (at::GradMode::is_enabled())
-    for (const Tensor* t : inputs)
-      if (t->defined() && t->requires_grad()) return true;
+  for (const Tensor* t : inputs)
+    if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 void first_derivatives_only(const char* what) {
@@ -1341,8 +1342,8 @@ struct GatedScan {
     s.x = kernel_operand(x, io);
     s.gate = kernel_operand(gate, io);
     s.in_gate = kernel_operand(in_gate, io);
-    s.A = f32c(A.resolve_neg());
-    s.h0 = h0.defined() ? f32c(h0.resolve_neg()) : h0;
+    s.A = f32c(in_memory(A));
+    s.h0 = f32c(in_memory(h0));
     s.seq = cast(seq, at::kInt);
     s.normalize = normalize;
     s.reverse = reverse;
@@ -1459,7 +1460,7 @@ struct GatedScanFn : public Function<GatedScanFn> {
     s.normalize = in->normalize;
     s.reverse = in->reverse;
     const c10::DeviceGuard guard(s.x.device());
-    const Tensor dy = kernel_operand(grads[0], s.x.scalar_type()), dlast = in->last && grads[1].defined() ? f32c(grads[1].resolve_neg()) : Tensor();
+    const Tensor dy = kernel_operand(grads[0], s.x.scalar_type()), dlast = in->last && grads[1].defined() ? f32c(in_memory(grads[1])) : Tensor();
     variable_list out(NIN + 4);
     if (!dy.defined() && !dlast.defined()) return out;
     Tensor g[NIN];
@@ -1562,7 +1563,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, con
   py::gil_scoped_release release;
   const c10::DeviceGuard guard(x.device());
   const at::ScalarType io = kernel_type(x.scalar_type());
-  const Tensor xk = kernel_operand(x, io), gk = kernel_operand(gate, io), ik = kernel_operand(in_gate, io), Ak = f32c(A.resolve_neg()),
+  const Tensor xk = kernel_operand(x, io), gk = kernel_operand(gate, io), ik = kernel_operand(in_gate, io), Ak = f32c(in_memory(A)),
                ak = at.defined() ? at.contiguous() : at;
   const Tensor y = fresh(x.sizes(), x, io);
   if (x.numel() == 0) return cast(y, x.scalar_type());
@@ -1608,7 +1609,7 @@ struct Rotary {
       r.w[0] = kernel_operand(wq, wt);
       r.w[1] = kernel_operand(wk, wt);
     }
-    r.table = f32c(table.resolve_neg());
+    r.table = f32c(in_memory(table));
     r.pos = pos;
     r.eps = eps;
     r.inter = inter;

@@ -1433,7 +1433,7 @@ static int gscan_sizes(const issm_gated_scan_args* a) {
   if (!a) return fail(ISSM_E_NULL, "gated_scan: args is NULL");
   if (a->batch < 1 || a->seqlen < 1 || a->channels < 1 || a->seqlen > (1 << 30))
     return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d", a->batch, a->seqlen, a->channels);
-  if ((int64_t)a->batch * gscan_blocks(a->channels) * gscan_tiles(a->seqlen, 1) >= (1 << 24))
+  if ((int64_t)a->batch * gscan_blocks(a->channels) * gscan_tiles(a->seqlen, 1) >= (1 << 24) || (int64_t)a->batch * gscan_blocks(a->channels) >= (1 << 22))
     return fail(ISSM_E_SHAPE, "gated_scan: batch=%d seqlen=%d channels=%d are too many tiles", a->batch, a->seqlen, a->channels);
   if (a->dtype != ISSM_F32 && a->dtype != ISSM_BF16) return fail(ISSM_E_DTYPE, "gated_scan: dtype %d", a->dtype);
   if (a->flags & ~(ISSM_GS_NORMALIZE | ISSM_GS_REVERSE)) return fail(ISSM_E_UNSUPPORTED, "gated_scan: flags 0x%x", a->flags);

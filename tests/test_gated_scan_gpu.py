@@ -419,3 +419,126 @@ def test_step_tells_what_saved_its_state_and_is_captured():
         assert torch.equal(y, y0)
     with torch.inference_mode():
         gated_scan_step(g["x"], g["gate"], g["A"], torch.zeros(4, 8, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------- ways through the kernels
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C,packed,reverse", [(520, 130, 8, 0, False), (520, 57, 8, 3, True), (300, 113, 72, 2, False), (515, 1, 4, 0, False), (530, 56, 7, 2, False)])
+def test_rows_that_fill_the_gpu(B, L, C, packed, reverse, dtype):
+    """Many rows, one workgroup each from the first tile to the last; an odd width takes the other addresses."""
+    case = make(B, L, C, dtype, seed=L, packed=packed)
+    check(run(*case, reverse=reverse), ref(*case, reverse=reverse))
+
+
+@pytest.mark.parametrize("L", [55, 56, 57, 111, 112, 113, 223, 224, 225, 448, 449])
+@pytest.mark.parametrize("C", [62, 64, 66])
+def test_ends_of_tiles(L, C):
+    """Lengths and widths to both sides of what a tile takes, forward and backward."""
+    case = make(2, L, C, torch.bfloat16, seed=L, packed=1)
+    check(run(*case), ref(*case))
+
+
+def test_long_rows():
+    """20000 tokens through some 180 tiles of 112 and 360 of 56, on many workgroups, twice: the oracle's values, and the same bits."""
+    case = make(2, 20000, 6, torch.float32, packed=2)
+    got = run(*case)
+    check(got, ref(*case))
+    again = run(*case)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_same_values_by_all_addresses(dtype):
+    """Rows at odd places and rows too far apart for 32 bits: what aligned rows give, bit for bit, states and their gradients too."""
+    from dest3d_amd import gated_scan
+    B, L, C = 2, 150, 64
+    d, dy, dlast = make(B, L, C, dtype)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    want = run(d, dy, dlast)
+
+    def moved(t, token, start):
+        wide = torch.empty(start + B * L * token, dtype=dtype, device="cuda")
+        v = wide.as_strided((B, L, C), (L * token, token, 1), start)
+        v.copy_(t)
+        return v
+
+    for token, start in ((C + 3, 1), (C + 2, 0), (5_000_000, 0) if dtype == torch.bfloat16 else (C + 1, 3)):
+        x = moved(g["x"], token, start).requires_grad_()
+        gate = moved(g["gate"], C + 2, 2).requires_grad_()
+        y, last = gated_scan(x, gate, g["A"], in_gate=g["in_gate"], initial_states=g["initial_states"], return_final_states=True)
+        dx, dgate = torch.autograd.grad((y, last), (x, gate), (dy.cuda(), dlast.cuda()))
+        assert torch.equal(y, want["y"]) and torch.equal(last, want["last"]) and torch.equal(dx, want["dx"]) and torch.equal(dgate, want["dgate"])
+        del x, gate
+
+
+def test_offsets_beyond_32_bits():
+    """Tokens, rows and slots more than 2^31 elements apart."""
+    from dest3d_amd import gated_scan, gated_scan_step
+    far = 2 ** 31 + 64
+    wide = torch.empty(far + 4096, dtype=torch.bfloat16, device="cuda")
+    A = -torch.rand(64, device="cuda") - 0.03
+    for strides in ((0, far), (far, 64)):
+        n = (1, 2) if strides[0] == 0 else (2, 2)
+        x = wide.as_strided((*n, 64), (*strides, 1))
+        x.copy_(torch.randn(*n, 64))
+        gate = torch.randn(*n, 64, device="cuda").bfloat16()
+        assert torch.equal(gated_scan(x, gate, A), gated_scan(x.contiguous(), gate, A))
+        assert torch.equal(gated_scan(x, gate, A, reverse=True), gated_scan(x.contiguous(), gate, A, reverse=True))
+    pool = torch.empty(far + 4096, dtype=torch.float32, device="cuda").as_strided((2, 64), (far, 1))
+    pool.copy_(torch.randn(2, 64))
+    small, at = pool.contiguous(), torch.tensor([1, 0], device="cuda")
+    x = torch.randn(2, 64, device="cuda")
+    assert torch.equal(gated_scan_step(x, x, A, pool, state_indices=at), gated_scan_step(x, x, A, small, state_indices=at))
+    assert torch.equal(pool, small)
+
+
+def test_refusals():
+    from dest3d_amd import gated_scan, gated_scan_step
+    x, A = torch.zeros(2, 5, 8, device="cuda"), torch.full((8,), -1.0, device="cuda")
+    ids = torch.zeros(2, 5, dtype=torch.int32, device="cuda")
+    for kw in (dict(x=x[0]), dict(gate=x[:, :4]), dict(in_gate=x[..., :4]), dict(A=A[:4]), dict(A=A[None]), dict(initial_states=x[:, 0, :4]), dict(seq_idx=ids[:, :4])):
+        with pytest.raises(ValueError):
+            gated_scan(**{**dict(x=x, gate=x, A=A), **kw})
+    for kw in (dict(x=x.long()), dict(gate=x.int()), dict(A=A.long()), dict(seq_idx=ids.float()), dict(initial_states=ids[:, :1].expand(2, 8))):
+        with pytest.raises(TypeError):
+            gated_scan(**{**dict(x=x, gate=x, A=A), **kw})
+    for kw in (dict(gate=x.cpu()), dict(A=A.cpu()), dict(seq_idx=ids.cpu())):
+        with pytest.raises(RuntimeError, match="all operands must be on"):
+            gated_scan(**{**dict(x=x, gate=x, A=A), **kw})
+    t, s = x[:, 0], torch.zeros(3, 8, device="cuda")
+    at = torch.tensor([0, 2], device="cuda")
+    for kw in (dict(x=x), dict(gate=t[:1]), dict(A=A[:4]), dict(state=s[:, :4]), dict(state_indices=at[:1]), dict(state_indices=None)):
+        with pytest.raises(ValueError):
+            gated_scan_step(**{**dict(x=t, gate=t, A=A, state=s, state_indices=at), **kw})
+    for kw in (dict(state=s.double()), dict(state=s.bfloat16()), dict(state_indices=at.float()), dict(state_indices=at.to(torch.int16))):
+        with pytest.raises(TypeError):
+            gated_scan_step(**{**dict(x=t, gate=t, A=A, state=s, state_indices=at), **kw})
+    for state in (s[:1].expand(3, 8), torch.zeros(8, 3, device="cuda").t()):     # slots that overlap, channels apart
+        with pytest.raises(AssertionError):
+            gated_scan_step(t, t, A, state, state_indices=at)
+    with pytest.raises(RuntimeError, match="no backward"):
+        gated_scan_step(t.clone().requires_grad_(), t, A, s, state_indices=at)
+    with torch.no_grad():
+        gated_scan_step(t.clone().requires_grad_(), t, A, s, state_indices=at)
+
+
+def test_modes():
+    """Inference mode, lazy negations, and forward derivatives, which there are none of."""
+    from dest3d_amd import gated_scan, qk_norm_rotary, rotary, rotary_table
+    d, _, _ = make(2, 60, 8, torch.float32)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    want = gated_scan(**g)
+    q, w, tab = torch.randn(1, 9, 2, 32, device="cuda"), torch.rand(32, device="cuda"), rotary_table(9, 32)
+    turned = rotary(q, None, tab)
+    with torch.inference_mode():
+        assert torch.equal(gated_scan(**g), want) and torch.equal(rotary(q, None, tab), turned)
+    lazy = torch.complex(g["x"], -g["x"]).conj().imag
+    assert lazy.is_neg() and torch.equal(gated_scan(**{**g, "x": lazy}), want)
+    lazy = torch.complex(q, -q).conj().imag
+    assert lazy.is_neg() and torch.equal(rotary(lazy, None, tab), turned)
+    import torch.autograd.forward_ad as fwAD
+    with fwAD.dual_level():
+        for call in (lambda: gated_scan(fwAD.make_dual(g["x"], g["x"]), g["gate"], g["A"]), lambda: rotary(fwAD.make_dual(q, q), None, tab),
+                     lambda: qk_norm_rotary(fwAD.make_dual(q, q), None, w, None, tab)):
+            with pytest.raises(RuntimeError):
+                call()

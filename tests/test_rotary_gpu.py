@@ -332,3 +332,45 @@ def test_a_layer_of_them(dtype):
     assert rel(out.detach(), outr.detach()) <= lim[0]
     for k, a, b_ in zip(d, grads, want):
         assert a.dtype == d[k].dtype and rel(a, b_) <= lim[1], (k, rel(a, b_))
+
+
+def test_offsets_beyond_32_bits_and_many_tokens():
+    from dest3d_amd import qk_norm_rotary, rotary
+    far, tab, w = 2 ** 31 + 64, table(9, 64).cuda(), torch.ones(64, device="cuda")
+    wide = torch.empty(far + 4096, dtype=torch.bfloat16, device="cuda")
+    for shape, strides in (((1, 1, 2, 64), (0, 0, far, 1)), ((1, 2, 1, 64), (0, far, 64, 1)), ((2, 1, 1, 64), (far, 64, 64, 1))):
+        q = wide.as_strided(shape, strides)
+        q.copy_(torch.randn(shape))
+        assert torch.equal(rotary(q, None, tab), rotary(q.contiguous(), None, tab))
+        a, b = (t.detach().requires_grad_() for t in (q, q.contiguous()))
+        grads = [torch.autograd.grad(qk_norm_rotary(t, None, w, None, tab), t, b.detach())[0] for t in (a, b)]
+        assert torch.equal(*grads)
+    # enough tokens of one head for several of them a wave
+    case = make(3, 30000, 1, 1, 16, 16, torch.float32, rows=30000)
+    for norm in (False, True):
+        check(run(*case, norm, True), ref(*case, norm, True))
+
+
+def test_refusals():
+    from dest3d_amd import qk_norm_rotary, rotary
+    q, k, tab, w = torch.zeros(2, 5, 4, 16, device="cuda"), torch.zeros(2, 5, 2, 16, device="cuda"), table(5, 16).cuda(), torch.ones(16, device="cuda")
+    pos = torch.zeros(2, 5, dtype=torch.int32, device="cuda")
+    for kw in (dict(q=q[0]), dict(k=k[:1]), dict(k=k[:, :4]), dict(k=k[..., :8]), dict(table=tab[:, :7]), dict(table=table(5, 18).cuda()), dict(table=tab[0]), dict(table=tab[:4]),
+               dict(positions=pos[:, :4]), dict(positions=pos[:1]), dict(positions=pos[..., None]), dict(table=tab[:0], positions=pos)):
+        with pytest.raises(ValueError):
+            rotary(**{**dict(q=q, k=k, table=tab), **kw})
+    for kw in (dict(q=q.long()), dict(k=k.int()), dict(table=tab.long()), dict(positions=pos.float()), dict(positions=pos.to(torch.int16))):
+        with pytest.raises(TypeError):
+            rotary(**{**dict(q=q, k=k, table=tab), **kw})
+    for kw in (dict(k=k.cpu()), dict(table=tab.cpu()), dict(positions=pos.cpu())):
+        with pytest.raises(RuntimeError, match="all operands must be on"):
+            rotary(**{**dict(q=q, k=k, table=tab), **kw})
+    with pytest.raises(AssertionError, match="no gradient"):
+        rotary(q, k, tab.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="1024"):
+        rotary(torch.zeros(1, 1, 1, 1026, device="cuda"), None, tab)
+    for kw in (dict(q_weight=w[:8]), dict(k_weight=w[None])):
+        with pytest.raises(ValueError):
+            qk_norm_rotary(**{**dict(q=q, k=k, q_weight=w, k_weight=w, table=tab), **kw})
+    with pytest.raises(TypeError):
+        qk_norm_rotary(q, k, w.long(), w, tab)

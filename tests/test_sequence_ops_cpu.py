@@ -50,7 +50,7 @@ def _scan(lib, **kw):
 
 @pytest.mark.parametrize("kw,code,text", [
     (dict(batch=0), -2, "batch=0"), (dict(seqlen=-1), -2, "seqlen=-1"), (dict(channels=0), -2, "channels=0"), (dict(seqlen=2 ** 31 - 1), -2, ""),
-    (dict(batch=2 ** 30, seqlen=2 ** 30), -2, "too many"), (dict(dtype=2), -4, "dtype"), (dict(flags=8), -5, "flags"), (dict(x=None), -1, ""), (dict(gate=None), -1, ""),
+    (dict(batch=2 ** 30, seqlen=2 ** 30), -2, "too many"), (dict(batch=2 ** 22, seqlen=1), -2, "too many"), (dict(dtype=2), -4, "dtype"), (dict(flags=8), -5, "flags"), (dict(x=None), -1, ""), (dict(gate=None), -1, ""),
     (dict(A=None), -1, ""), (dict(y=None), -1, "y is NULL"), (dict(x_stride=(-1, 8)), -3, "stride"), (dict(gate_stride=(0, -8)), -3, "stride"),
     (dict(in_gate=FAKE, in_gate_stride=(-8, 8)), -3, "stride"), (dict(seq_idx=FAKE, seq_idx_stride=(4, -1)), -3, "stride")])
 def test_scan_refuses(lib, kw, code, text):
