@@ -586,7 +586,7 @@ __global__ __launch_bounds__(1024) void k_gscan_sum(const float* part, int rows,
 }
 
 // One token a row, four channels a thread.  Rows whose slot is none of the pool's give zeros and touch no state.  Several rows of one slot are
-// taken in their order, by the first of them: a wave looks over all rows' slots, 256 requested at a time.
+// taken in their order, by the first of them: a workgroup looks over all rows' slots, each of its waves over a quarter of them.
 // Bound by its bytes: 512 rows of 4096 channels bf16 in a pool, 33.6 MB.
 template <bool BF>
 struct Four {   // the channels that there are of four
@@ -628,23 +628,34 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
   old.load(state, c0, n);
   int next = p.rows;   // the next row of the slot
   if (p.at) {
-    bool before = false;
-    for (int q = 0; q < p.rows; q += 256) {
-      long s[4];
+    __shared__ int first_of[4], next_of[4];
+    const int wave = threadIdx.x >> 6;
+    int first = p.rows;
+    for (int q = 64 * wave; q < p.rows; q += 512) {
+      long s[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = slot_of(min(q + 64 * i + lane, p.rows - 1));
+      for (int i = 0; i < 2; ++i) s[i] = slot_of(min(q + 256 * i + lane, p.rows - 1));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = q + 64 * i + lane;
+      for (int i = 0; i < 2; ++i) {
+        const int r = q + 256 * i + lane;
         const bool same = r < p.rows && s[i] == slot;
-        before = before || (same && r < row);
+        first = same ? min(first, r) : first;
         next = same && r > row ? min(next, r) : next;
       }
     }
-    if (__any(before)) return;
-    if (__any(next < p.rows))
+    if (__any(first < p.rows))
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o, 64));
+      for (int o = 32; o > 0; o >>= 1) {
+        first = min(first, __shfl_xor(first, o, 64));
+        next = min(next, __shfl_xor(next, o, 64));
+      }
+    if (lane == 0) {
+      first_of[wave] = first;
+      next_of[wave] = next;
+    }
+    __syncthreads();
+    if (min(min(first_of[0], first_of[1]), min(first_of[2], first_of[3])) < row) return;
+    next = min(min(next_of[0], next_of[1]), min(next_of[2], next_of[3]));
   }
   float h[4];
 #pragma unroll
