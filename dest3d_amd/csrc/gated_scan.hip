@@ -11,6 +11,12 @@
 // A workgroup takes tiles of GS_TT * S tokens and GS_CG * V channels: a thread V channels of S tokens one behind the other, whose map
 // h -> P h + H it leaves in LDS.  A wave without tokens of its own, a channel a lane, joins the maps of the tile and gives every thread its first
 // state; with the tokens' requests out of its way its looks at other tiles come back at once (a wave's loads return in their order).
+// GS_CG * V = 64 channels are rows' pieces of 128 bytes in bf16: with half of that a row of
+// 131072 tokens of 2048 channels, 585 us at the time, took 715.
+//
+// Bound by bytes, and where rows are few by waiting for the states in front: bf16, 16 x 4096 tokens of 2048 channels (rows walked) 246 us forward,
+// 4.4 TB/s, and 426 backward, 4.4; 8 x 4096 (rows shared by two and three) 136 and 254, 4.0 and 3.7; 1 x 131072 (by sixteen and 24) 529, 4.1, and
+// 1126, 3.3: copies of it that did not wait took 465 and 852.  (Launches that clear the words and sum dA included.)  A copy of 1 GiB: 5.1 TB/s.
 #include "gated_scan_dev.h"
 
 // (every multiply-add is written as one: the forms of a kernel that do the same sums are to give the same bits)
@@ -587,7 +593,8 @@ __global__ __launch_bounds__(1024) void k_gscan_sum(const float* part, int rows,
 
 // One token a row, four channels a thread.  Rows whose slot is none of the pool's give zeros and touch no state.  Several rows of one slot are
 // taken in their order, by the first of them: a workgroup looks over all rows' slots, each of its waves over a quarter of them.
-// Bound by its bytes: 512 rows of 4096 channels bf16 in a pool, 33.6 MB.
+// Bound by its bytes where rows are many (512 rows of 4096 channels bf16, 33.6 MB, 7.8 us, 9.2 with their slots
+// named; 10.0 with every wave looking at all of them), by a launch and two trips to memory where they are few (one row of 2048 2.5 us).
 template <bool BF>
 struct Four {   // the channels that there are of four
   Piece<BF, 4> m;

@@ -6,7 +6,9 @@
 // A lane owns V pairs of a row (one head of one token), so that a rotation is its own affair; LPR lanes, a power of two, share a row and
 // its sums.  The 64 / LPR rows that a wave has at a time are `group` heads of 64 / LPR / group tokens; it goes on to their other heads, or, where
 // a token has no more, to other tokens, and asks for NB of its rows before it works on the first.  Angles and weights stay with the lane.
-// Rows are bound by their bytes, read and written once.
+// Rows are bound by their bytes, read and written once: bf16, 16384 tokens of 32 and 8 heads of 128, with the norm, 70 us, 4.8 TB/s (a copy
+// of 256 MiB 5.4); 65536 of 16 and 4, alone, 130 us, 5.2; the norm's gradients of 16384 tokens of 16 and 4, 252 MB, 53 us behind other work and 47
+// over and over, 4.8 and 5.4.  Rows with angles and weights asked for each by itself, four at a time: 97, 151 and 63 us.
 #include "rotary_dev.h"
 
 // (every multiply-add is written as one: the forms of a kernel that do the same sums are to give the same bits)
