@@ -764,9 +764,24 @@ static void launch_step(const GStepP& p, bool nrm, hipStream_t st) {
   if (p.i) nrm ? k_gscan_step<BF, true, true><<<grid, 256, 0, st>>>(p) : k_gscan_step<BF, true, false><<<grid, 256, 0, st>>>(p);
   else nrm ? k_gscan_step<BF, false, true><<<grid, 256, 0, st>>>(p) : k_gscan_step<BF, false, false><<<grid, 256, 0, st>>>(p);
 }
+// Rows with slots go in launches of at most GS_STEP_ROWS, one behind the other: a row looks at its launch's slots only, so that the looking grows with
+// the rows and not with their square, and a slot's rows stay in their order.  (8192 rows bf16 of 4096 channels by 1024, 2048, 4096, 8192: 169, 162,
+// 174, 217 us; of 256: 43, 34, 36, 44.)
+constexpr int GS_STEP_ROWS = 2048;
 int launch_gscan_step(GStepP p, bool bf, bool nrm, hipStream_t st) {
   p.ncb = (p.C + 1023) / 1024;
-  bf ? launch_step<true>(p, nrm, st) : launch_step<false>(p, nrm, st);
+  const int rows = p.rows, most = p.at ? GS_STEP_ROWS : rows;
+  const long size = bf ? 2 : 4, index = p.at64 ? 8 : 4;
+  auto on = [](auto*& q, long bytes) { q = q ? (std::remove_reference_t<decltype(q)>)((const char*)q + bytes) : q; };
+  for (int r = 0; r < rows; r += most) {
+    p.rows = min(most, rows - r);
+    bf ? launch_step<true>(p, nrm, st) : launch_step<false>(p, nrm, st);
+    on(p.x, most * p.xs * size);
+    on(p.g, most * p.gs * size);
+    on(p.i, most * p.is * size);
+    on(p.at, most * index);
+    on(p.y, (long)most * p.C * size);
+  }
   return (int)hipGetLastError();
 }
 

@@ -542,3 +542,31 @@ def test_modes():
                      lambda: qk_norm_rotary(fwAD.make_dual(q, q), None, w, None, tab)):
             with pytest.raises(RuntimeError):
                 call()
+
+
+@pytest.mark.parametrize("dtype,index,C", [(torch.float32, torch.int64, 5), (torch.bfloat16, torch.int32, 8)])
+def test_step_of_many_rows(dtype, index, C):
+    """More rows than a launch looks over: those of one slot still in their order, whichever launch they are in."""
+    from dest3d_amd import gated_scan_step
+    rows, slots = 4099, 1500
+    d, _, _ = make(1, rows, C, dtype)
+    x, gate, in_gate, A = d["x"][0], d["gate"][0], d["in_gate"][0], d["A"]
+    wide = torch.cat([x, gate, in_gate], 1).cuda()      # rows that lie apart
+    gen = torch.Generator().manual_seed(5)
+    at = torch.randint(-1, slots, (rows,), generator=gen)
+    at[[0, 2047, 2048, 4096, 4098]] = 11
+    pool = torch.randn(slots, C, generator=gen)
+    got = pool.cuda()
+    y = gated_scan_step(wide[:, :C], wide[:, C:2 * C], A.cuda(), got, in_gate=wide[:, 2 * C:], state_indices=at.to(index).cuda())
+    state, want = pool.double(), torch.zeros(rows, C, dtype=torch.float64)
+    turn = torch.zeros(rows, dtype=torch.long)           # a row's place among those of its slot
+    seen = {}
+    for r, s in enumerate(at.tolist()):
+        turn[r] = seen[s] = seen.get(s, -1) + 1
+    for n in range(int(turn.max()) + 1):
+        r = ((turn == n) & (at >= 0)).nonzero()[:, 0]
+        h, _ = R.gated_scan(x[r][:, None].double(), gate[r][:, None].double(), A.double(), in_gate[r][:, None].double(), state[at[r]])
+        state[at[r]] = want[r] = h[:, 0]
+    # (a value's states are off by 7e-6 of their size, about 1 to 4 here; bf16 by half a step on top)
+    assert ((y.double().cpu() - want).abs() <= 3e-5 + (STEP * want.abs() if dtype == torch.bfloat16 else 0.0)).all()
+    assert ((got.double().cpu() - state).abs() <= 3e-5).all() and not y[at.cuda() < 0].any()
