@@ -1321,6 +1321,12 @@ std::vector<Tensor> scan_layer(const Tensor& in_key, const Tensor& in_query, con
 // (a tensor that is the lazy negation of its memory is computed first)
 Tensor in_memory(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 Tensor kernel_operand(const Tensor& t, at::ScalarType type) { return io_cast(in_memory(t), type); }
+// The type in which a call reads operands that go together: bf16 where all of them are, or those in float32 would be rounded
+at::ScalarType common_type(std::initializer_list<const Tensor*> operands) {
+  for (const Tensor* t : operands)
+    if (t->defined() && t->scalar_type() != at::kBFloat16) return at::kFloat;
+  return at::kBFloat16;
+}
 // whether a call is a node's: to be differentiated, or (as the nodes say by an error) carrying a forward derivative that would be lost
 bool recorded(std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
@@ -1338,7 +1344,7 @@ struct GatedScan {
   static GatedScan make(const Tensor& x, const Tensor& gate, const Tensor& A, const Tensor& in_gate, const Tensor& h0, const Tensor& seq,
                         bool normalize, bool reverse) {
     GatedScan s;
-    const at::ScalarType io = kernel_type(x.scalar_type());
+    const at::ScalarType io = common_type({&x, &gate, &in_gate});
     s.x = kernel_operand(x, io);
     s.gate = kernel_operand(gate, io);
     s.in_gate = kernel_operand(in_gate, io);
@@ -1562,7 +1568,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, con
     raise_py(PyExc_RuntimeError, "gated_scan_step has no backward: call it under torch.no_grad(), or gated_scan");
   py::gil_scoped_release release;
   const c10::DeviceGuard guard(x.device());
-  const at::ScalarType io = kernel_type(x.scalar_type());
+  const at::ScalarType io = common_type({&x, &gate, &in_gate});
   const Tensor xk = kernel_operand(x, io), gk = kernel_operand(gate, io), ik = kernel_operand(in_gate, io), Ak = f32c(in_memory(A)),
                ak = at.defined() ? at.contiguous() : at;
   const Tensor y = fresh(x.sizes(), x, io);
@@ -1601,7 +1607,7 @@ struct Rotary {
   static Rotary make(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& table, const Tensor& pos, double eps,
                      bool inter) {
     Rotary r;
-    const at::ScalarType io = kernel_type(q.scalar_type());
+    const at::ScalarType io = common_type({&q, &k});
     r.x[0] = kernel_operand(q, io);
     r.x[1] = kernel_operand(k, io);
     if (wq.defined()) {

@@ -12,12 +12,13 @@ def gated_scan(x, gate, A, in_gate=None, initial_states=None, seq_idx=None, norm
     r = sigmoid(gate), a = exp(A r), u = sigmoid(in_gate) x (x without in_gate), h_t = a_t h_{t-1} + sqrt(1 - a_t^2) u_t
 
     Argument:
-        x: (batch, seqlen, channels), float32 or bfloat16 (other types are computed in float32 and returned in their own)
+        x: (batch, seqlen, channels), float32 or bfloat16 (other types are computed in float32 and returned in their
+            own; so is all of a call whose x, gate and in_gate are not all bfloat16)
         gate: (batch, seqlen, channels), before the sigmoid
         A: (channels,) logarithm of the decay at a full gate, <= 0
         in_gate: (batch, seqlen, channels), before the sigmoid, or None
         initial_states: (batch, channels) or None
-        seq_idx: (batch, seqlen) integer ids of the sequences packed into a row, or None.  Every change of id is a cut that nothing
+        seq_idx: (batch, seqlen) integer ids (compared as int32) of the sequences packed into a row, or None.  Every change of id is a cut that nothing
             passes; initial_states count as id 0, as in ISSM_chunk_scan_combined.
         normalize: without it u_t enters as it is (and A may be positive)
         reverse: from the last token to the first; initial_states and the final states are then behind and before the row

@@ -47,7 +47,8 @@ def rotary_table(length, dim, base=10000.0, scaling=None, factor=1.0, original_l
 def rotary(q, k, table, positions=None, interleaved=False):
     """
     Argument:
-        q: (batch, seqlen, heads, headdim), k: (batch, seqlen, kv_heads, headdim) or None; features contiguous, other strides as they are
+        q: (batch, seqlen, heads, headdim), k: (batch, seqlen, kv_heads, headdim) or None; features contiguous, other strides as they are.
+            bfloat16 where both are, else computed in float32; each is returned in its own type
         table: (rows, rot) of rotary_table; the first rot <= headdim features of a head are turned, the others returned as they are
         positions: (batch, seqlen) or (seqlen,) int32 or int64, rows of the table, or None: 0, 1, ... along the sequence.  A position
             outside the table makes its token's turned features NaN.

@@ -570,3 +570,18 @@ def test_step_of_many_rows(dtype, index, C):
     # (a value's states are off by 7e-6 of their size, about 1 to 4 here; bf16 by half a step on top)
     assert ((y.double().cpu() - want).abs() <= 3e-5 + (STEP * want.abs() if dtype == torch.bfloat16 else 0.0)).all()
     assert ((got.double().cpu() - state).abs() <= 3e-5).all() and not y[at.cuda() < 0].any()
+
+
+@pytest.mark.parametrize("wide", [("gate",), ("in_gate",), ("x",), ("gate", "in_gate")])
+def test_operands_of_two_types(wide):
+    """An operand in float32 beside others in bfloat16 is not rounded to theirs: what is returned in float32 is as exact as if all were."""
+    from dest3d_amd import gated_scan_step
+    d, dy, dlast = make(2, 150, 20, torch.bfloat16, seed=3)
+    for k in wide:
+        d[k] = torch.randn(2, 150, 20, generator=torch.Generator().manual_seed(len(k)))
+    check(run(d, dy.to(d["x"].dtype), dlast), ref(d, dy, dlast))
+    one = {k: d[k][:, 0] for k in ("x", "gate", "in_gate")}
+    pool = d["initial_states"].cuda()
+    gated_scan_step(one["x"].cuda(), one["gate"].cuda(), d["A"].cuda(), pool, in_gate=one["in_gate"].cuda())
+    want, _ = R.gated_scan(*(one[k][:, None].double() for k in ("x", "gate")), d["A"].double(), one["in_gate"][:, None].double(), d["initial_states"].double())
+    assert (pool.double().cpu() - want[:, 0]).norm() <= FP32["y"] * want.norm()

@@ -374,3 +374,12 @@ def test_refusals():
             qk_norm_rotary(**{**dict(q=q, k=k, q_weight=w, k_weight=w, table=tab), **kw})
     with pytest.raises(TypeError):
         qk_norm_rotary(q, k, w.long(), w, tab)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("wide", ["q", "k"])
+def test_sides_of_two_types(wide, norm):
+    """A side in float32 beside one in bfloat16 is not rounded to the other's type."""
+    d, dq, dk = make(2, 30, 4, 2, 64, 48, torch.bfloat16)
+    d[wide] = torch.randn(d[wide].shape, generator=torch.Generator().manual_seed(4))
+    check(run(d, dq.to(d["q"].dtype), dk.to(d["k"].dtype), norm, False), ref(d, dq, dk, norm, False))
