@@ -1786,7 +1786,7 @@ std::vector<Tensor> rotary(const Tensor& q, const MaybeTensor& k_, const MaybeTe
   require_shape(table.dim() == 2 && table.size(1) >= 2 && table.size(1) % 2 == 0 && table.size(1) <= D && table.size(0) >= 1, "table",
                 "(positions, turned features) with an even number of at most headdim features", table);
   require_type(at::isFloatingType(table.scalar_type()), "table", "of a floating type", table);
-  require(!(at::GradMode::is_enabled() && table.requires_grad()), "table has no gradient: detach it");
+  require(!(at::GradMode::is_enabled() && table.requires_grad()) && !table._fw_grad(0).defined(), "table has no gradient: detach it");
   if (pos.defined()) {
     require_shape((pos.dim() == 2 && pos.size(0) == B && pos.size(1) == L) || (pos.dim() == 1 && pos.size(0) == L), "positions",
                   "(batch, seqlen) or (seqlen,)", pos);

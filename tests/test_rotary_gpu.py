@@ -383,3 +383,10 @@ def test_sides_of_two_types(wide, norm):
     d, dq, dk = make(2, 30, 4, 2, 64, 48, torch.bfloat16)
     d[wide] = torch.randn(d[wide].shape, generator=torch.Generator().manual_seed(4))
     check(run(d, dq.to(d["q"].dtype), dk.to(d["k"].dtype), norm, False), ref(d, dq, dk, norm, False))
+
+def test_table_without_forward_derivative():
+    import torch.autograd.forward_ad as fwAD
+    from dest3d_amd import rotary
+    q, tab = torch.zeros(1, 5, 2, 16, device="cuda"), table(5, 16).cuda()
+    with fwAD.dual_level(), pytest.raises(AssertionError, match="no gradient"):
+        rotary(q, None, fwAD.make_dual(tab, tab))
