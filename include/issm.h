@@ -764,7 +764,7 @@ typedef struct issm_gated_scan_args {
   void* din_gate;
   float* dA;
   float* dh0;
-  void* workspace; /* 256-byte aligned */
+  void* workspace; /* 16-byte aligned */
   size_t workspace_bytes;
   void* stream;
 } issm_gated_scan_args;
