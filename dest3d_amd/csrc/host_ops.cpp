@@ -6,6 +6,7 @@
 // kernels (and, for the layer's four projections, in the tensor library's matrix products).
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/SavedTensorHooks.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
@@ -1538,6 +1539,12 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Tensor
   return out;
 }
 
+// (of two tensors with gaps in one allocation it cannot be told)
+bool shares_memory(const Tensor& a, const Tensor& b) {
+  const at::MemOverlapStatus s = at::get_overlap_status(a, b);
+  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+}
+
 Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, const Tensor& state, const MaybeTensor& in_gate_,
                        const MaybeTensor& at_, bool normalize) {
   const Tensor in_gate = opt(in_gate_), at = opt(at_);
@@ -1557,6 +1564,8 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, con
   const int64_t rows = x.size(0), C = x.size(1), slots = state.size(0);
   require((C <= 1 || state.stride(1) == 1) && (slots <= 1 || state.stride(0) >= C) && !state.is_neg(),
           "state must have contiguous channels and slots that do not overlap (it is updated in place)");
+  for (const Tensor* t : {&x, &gate, &A, &in_gate})
+    require(!t->defined() || !shares_memory(*t, state), "state must share no memory with the other operands (it is updated in place)");
   if (at.defined()) {
     require_shape(at.dim() == 1 && at.size(0) == rows, "state_indices", "(rows,)", at);
     require_type(is_index(at), "state_indices", "int32 or int64", at);

@@ -37,7 +37,7 @@ def gated_scan_step(x, gate, A, state, in_gate=None, state_indices=None, normali
 
     Argument:
         x, gate, in_gate: (rows, channels), A: (channels,)
-        state: (slots, channels) float32, updated in place
+        state: (slots, channels) float32, updated in place; it shares no memory with the others
         state_indices: (rows,) int32 or int64, the slot of each row, or None: row r has slot r.  A row whose index is outside the
             slots (-1, say) gives zeros and touches no state; rows of one slot are taken in their order, as its tokens one
             behind the other.

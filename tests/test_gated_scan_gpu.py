@@ -585,3 +585,56 @@ def test_operands_of_two_types(wide):
     gated_scan_step(one["x"].cuda(), one["gate"].cuda(), d["A"].cuda(), pool, in_gate=one["in_gate"].cuda())
     want, _ = R.gated_scan(*(one[k][:, None].double() for k in ("x", "gate")), d["A"].double(), one["in_gate"][:, None].double(), d["initial_states"].double())
     assert (pool.double().cpu() - want[:, 0]).norm() <= FP32["y"] * want.norm()
+
+
+def test_step_refuses_its_state_as_an_input():
+    from dest3d_amd import gated_scan_step
+    pool, x, A = torch.randn(4, 8, device="cuda"), torch.randn(4, 8, device="cuda"), torch.full((8,), -1.0, device="cuda")
+    before = pool.clone()
+    for kw in (dict(x=pool), dict(gate=pool), dict(in_gate=pool), dict(A=pool[1]), dict(x=pool[1:], gate=x[1:], state=pool[:3])):
+        with pytest.raises(AssertionError, match="share no memory"):
+            gated_scan_step(**{**dict(x=x, gate=x, A=A, state=pool), **kw})
+    assert torch.equal(pool, before)
+    both = torch.randn(8, 8, device="cuda")    # (halves of one allocation are no overlap)
+    want = both[4:].clone()
+    y = gated_scan_step(both[:4], x, A, both[4:])
+    assert torch.equal(y, gated_scan_step(both[:4].clone(), x, A, want)) and torch.equal(both[4:], want)
+
+
+def test_kept_graphs_checkpoints_and_threads():
+    """A graph run backwards twice, a call computed again in its backward, and calls from several threads give the same bits."""
+    import threading
+    from torch.utils.checkpoint import checkpoint
+    from dest3d_amd import gated_scan
+    d, dy, _ = make(2, 300, 64, torch.float32)
+    g = {k: None if v is None else v.cuda() for k, v in d.items()}
+    leaves = [g[k].requires_grad_() for k in LEAVES]
+    dy = dy.cuda()
+
+    def call(x, gate, A, in_gate, h0):
+        return gated_scan(x, gate, A, in_gate, h0)
+
+    y = call(*leaves)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, dy)))
+    for reentrant in (False, True):
+        for t in leaves:
+            t.grad = None
+        checkpoint(call, *leaves, use_reentrant=reentrant).backward(dy)
+        assert all(torch.equal(a, t.grad) for a, t in zip(want, leaves))
+    same = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got = torch.autograd.grad(call(*leaves), leaves, dy)
+                torch.cuda.current_stream().synchronize()
+                same.append(all(torch.equal(a, b) for a, b in zip(want, got)))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True] * 15
