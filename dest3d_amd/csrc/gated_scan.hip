@@ -193,6 +193,22 @@ __global__ __launch_bounds__(256) void k_gscan_clear(uint4* p, long n) {
   for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
+// The row of a block of channels that a workgroup is of.  Where blocks of channels share cache lines (p.lines), an XCD's workgroups (every eighth one) take
+// rows that lie side by side, so that such a line is in one L2: 8 x 4096 x 1000 bf16 67 us forward and 145 backward, 83 and 169 without; 64 x 1024 x 1000
+// 126 and 228, 145 and 310; 4 x 5001 x 801 fp32, packed, 58 and 143, 67 and 155.  Where there are no such lines the other order is as fast or faster
+// (8 x 4096 x 2048 136 and 254, 136 and 254 side by side; 1 x 131072 x 2048 526 and 1126, 544 and 1165), and where a workgroup has hardly more than a tile:
+// XCDs do not get the same number of rows (3 x 3000 x 333 fp32 22 and 35, 22 and 38; 2 x 1000 x 290 11 and 16, 12 and 19).
+template <bool SHARED>
+__device__ __forceinline__ int chain_of(const GScanP& p) {
+  const unsigned rows = p.B * p.ncb, each = gridDim.x >> 3, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
+  if (!p.lines) return SHARED ? blockIdx.x % rows : blockIdx.x;
+  if (!SHARED || gridDim.x == rows) return xcd * each + min(xcd, gridDim.x & 7) + nth;
+  // (its rows in turn, the first and last of which may be another XCD's too; none is left out: rows that share their tiles so have GS_WG * NCU workgroups
+  // or more, an XCD more of them than rows)
+  const unsigned first = (xcd * rows) >> 3, mine = (((xcd + 1) * rows + 7) >> 3) - first;
+  return first + nth % mine;
+}
+
 // A row of a block of channels is one workgroup's, tile behind tile, or (SHARED) that of several: each takes the next tile that none has taken.
 // One barrier a tile.  From a tile's barrier to the next one's the maps' wave has its maps, looks for the state in front of it and gives the
 // threads theirs; meanwhile the others ask for the inputs of the tile behind it, finish the one before it, whose states lie there, and leave
@@ -254,7 +270,7 @@ template <bool BF, int V, int S, int IG, int NRM, bool SEQ, bool SHARED, bool BU
 __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) {
   constexpr int W = GS_CG * V, T = GS_TT * S;
   __shared__ FwdShared<W> sh;
-  const int chain = SHARED ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
+  const int chain = chain_of<SHARED>(p), cb = chain % p.ncb, b = chain / p.ncb;
   const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int k = 0;
   if (SHARED) {
@@ -428,7 +444,7 @@ template <bool BF, int V, int S, int IG, int NRM, bool SEQ, bool SHARED, bool BU
 __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(GScanP p) {
   constexpr int W = GS_CG * V, T = GS_TT * S;
   __shared__ BackMaps<W> m;
-  const int chain = SHARED ? blockIdx.x % (p.B * p.ncb) : blockIdx.x, cb = chain % p.ncb, b = chain / p.ncb;
+  const int chain = chain_of<SHARED>(p), cb = chain % p.ncb, b = chain / p.ncb;
   const int tid = threadIdx.x, cg = tid % GS_CG, tt = tid / GS_CG, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int k0 = 0;
   if (SHARED) {
@@ -742,6 +758,7 @@ int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st) 
   const int rows = p.B * p.ncb, S = back ? GS_S_BACK : GS_S_SHARED, share = sharing(rows, gscan_tiles(p.L, S), back);
   const bool buffers = behind_buffers(p, bf, back), shared = share > 1 || !buffers;
   p.nk = shared || back ? gscan_tiles(p.L, S) : gscan_tiles(p.L, GS_S_WALKED);
+  p.lines = (p.C * (bf ? 2L : 4L)) % 128 != 0 && (share == 1 || 2 * p.nk >= 3 * share);
   char* ws = (char*)workspace;
   if (back) {
     p.part = p.dA ? (float*)ws : nullptr;

@@ -13,7 +13,7 @@ constexpr int GS_S_SHARED = 4, GS_S_WALKED = 2, GS_S_BACK = 2, GS_TILE_BACK = GS
 
 struct GScanP {
   int B, L, C, ncb, nk, nb;       // ncb, nk, nb: blocks of channels, tiles of tokens, the backward's
-  bool nrm;
+  bool nrm, lines;                // lines: blocks of channels end inside cache lines
   const void *x, *g, *i, *dy;     // i, dy: or NULL
   long xb, xl, gb, gl, ib, il, dyb, dyl;   // strides of batch and token in elements; negative ones walk from the end
   const float *A, *h0, *dlast;    // (C); (B, C) or NULL

@@ -638,3 +638,23 @@ def test_kept_graphs_checkpoints_and_threads():
     for t in threads:
         t.join()
     assert same == [True] * 15
+
+
+@pytest.mark.parametrize("B,L,C,dtype,packed", [
+    (8, 6800, 66, torch.float32, 2), (7, 11000, 33, torch.float32, 0), (3, 15000, 130, torch.bfloat16, 3), (170, 240, 131, torch.float32, 2),
+    (513, 60, 34, torch.float32, 2), (260, 130, 70, torch.bfloat16, 0), (511, 300, 7, torch.bfloat16, 2), (5, 20, 33, torch.float32, 0)])
+def test_widths_that_share_cache_lines(B, L, C, dtype, packed):
+    """Rows in the order in which an XCD takes those side by side: numbers of rows that are multiples of eight and not, shared and walked.  The same
+    channels in rows of whole cache lines, which go in the other order, have the same bits; short ones are compared with the oracle too."""
+    d, dy, dlast = make(B, L, C, dtype, packed=packed)
+    got = run(d, dy, dlast)
+    more = -C % 64
+
+    def pad(k, t):
+        return t if t is None or k == "seq_idx" else torch.nn.functional.pad(t, (0, more), value=-0.5 if k == "A" else 0.0)
+
+    whole = run({k: pad(k, v) for k, v in d.items()}, pad("dy", dy), pad("dlast", dlast))
+    for k, v in got.items():
+        assert torch.isfinite(v).all() and torch.equal(v, whole[k][..., :C]), k
+    if L <= 130:
+        check(got, ref(d, dy, dlast))
