@@ -114,8 +114,9 @@ __device__ __forceinline__ void tile_map(const float (&sP)[TT][W], const float (
     P = cut || (SEQ && P < 0.0f) ? -1.0f : P * q;
   }
 }
+// What every segment starts from, in place of its H; returns the state behind them.
 template <bool SEQ, int TT, int W>
-__device__ __forceinline__ void tile_starts(const float (&sP)[TT][W], float (&sH)[TT][W], int w, bool back, float h) {
+__device__ __forceinline__ float tile_starts(const float (&sP)[TT][W], float (&sH)[TT][W], int w, bool back, float h) {
 #pragma unroll 8
   for (int i = 0; i < TT; ++i) {
     const int j = back ? TT - 1 - i : i;
@@ -123,7 +124,11 @@ __device__ __forceinline__ void tile_starts(const float (&sP)[TT][W], float (&sH
     sH[j][w] = h;
     h = SEQ && q < 0.0f ? f : fmaf(q, h, f);
   }
+  return h;
 }
+// Whether a tile's map is one in numbers.  Without beta decays may grow (A > 0): a product beyond fp32 would make a state of 0 NaN and small ones infinite.
+// The state behind such a tile is its segments', one behind the other, and the tiles behind it wait for that state.
+__device__ __forceinline__ bool in_range(float P, float H) { return __builtin_isfinite(P) && __builtin_isfinite(H); }
 
 template <int TT, int W>
 __device__ __forceinline__ void column_sum(const float (&s)[TT][W], int w, float* to) {
@@ -138,7 +143,7 @@ __device__ __forceinline__ bool decays(const float* from, float (&A)[V]) {
   bool near = true;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    A[v] = from[v];
+    A[v] = rate(from[v]);
     near = near && fabsf(A[v]) < GS_NEAR;
   }
   return __all(near);
@@ -146,7 +151,7 @@ __device__ __forceinline__ bool decays(const float* from, float (&A)[V]) {
 
 // The state in front of the o-th tile of a row (in the order of the walk), a channel a lane, from what the tiles in front of it have told:
 // the nearest state among the last GS_LOOK of them, and the maps from there on, in the order in which the tiles themselves apply
-// them -- whichever of the states is found, the bits are the same.
+// them -- whichever of the states is found, the bits are the same.  (A tile out of range tells no map: its state is waited for.)
 // Every wait ends: tiles are taken in their order (tickets), so the tiles in front of this one are on workgroups that run, and the first of them
 // that has not told its state waits for none that has not.  (After GS_POLLS looks, seconds, it would end with NaN: should memory be overwritten
 // from elsewhere, no workgroup stays.)
@@ -245,14 +250,18 @@ __device__ __forceinline__ void chain_fwd(const GScanP& p, FwdShared<W>& sh, int
     if (on) {
       float Pt, Ht;
       tile_map<SEQ, GS_TT, W>(m.P, m.H, w, false, Pt, Ht);
-      const bool cut_off = SEQ && Pt < 0.0f;
+      const bool cut_off = SEQ && Pt < 0.0f, whole = cut_off || in_range(Pt, Ht);
       if (SHARED && k > 0) {
-        tell(words + (long)k * 64, Ht, cut_off ? GS_STATE : map_bits(Pt));
+        if (whole) tell(words + (long)k * 64, Ht, cut_off ? GS_STATE : __float_as_uint(Pt));
         carry = look.back(words + (long)k * 64, k, first);
       }
-      const float behind = cut_off ? Ht : fmaf(Pt, carry, Ht);
-      if (SHARED && k + 1 < p.nk) tell(words + (long)k * 64, behind, GS_STATE);
-      tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, carry);
+      float behind = cut_off ? Ht : fmaf(Pt, carry, Ht);
+      if (SHARED && k + 1 < p.nk && whole) tell(words + (long)k * 64, behind, GS_STATE);
+      const float walked = tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, carry);
+      if (!whole) {
+        behind = walked;
+        if (SHARED && k + 1 < p.nk) tell(words + (long)k * 64, behind, GS_STATE);
+      }
       if (p.hs)
 #pragma unroll
         for (int i = 0; i < S / GS_S_BACK; ++i) {
@@ -420,14 +429,18 @@ __device__ __forceinline__ void chain_bwd(const GScanP& p, BackMaps<W>& m, int c
     if (on) {
       float Pt, Ct;
       tile_map<SEQ, GS_TT, W>(m.P, m.C, w, true, Pt, Ct);
-      const bool cut_off = SEQ && Pt < 0.0f;
+      const bool cut_off = SEQ && Pt < 0.0f, whole = cut_off || in_range(Pt, Ct);
       if (SHARED && o > 0) {
-        tell(words + (long)o * 64, Ct, cut_off ? GS_STATE : map_bits(Pt));
+        if (whole) tell(words + (long)o * 64, Ct, cut_off ? GS_STATE : __float_as_uint(Pt));
         carry = look.back(words + (long)o * 64, o, first);
       }
-      const float behind = cut_off ? Ct : fmaf(Pt, carry, Ct);
-      if (SHARED && o + 1 < p.nk) tell(words + (long)o * 64, behind, GS_STATE);
-      tile_starts<SEQ, GS_TT, W>(m.P, m.C, w, true, carry);
+      float behind = cut_off ? Ct : fmaf(Pt, carry, Ct);
+      if (SHARED && o + 1 < p.nk && whole) tell(words + (long)o * 64, behind, GS_STATE);
+      const float walked = tile_starts<SEQ, GS_TT, W>(m.P, m.C, w, true, carry);
+      if (!whole) {
+        behind = walked;
+        if (SHARED && o + 1 < p.nk) tell(words + (long)o * 64, behind, GS_STATE);
+      }
       tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, before);
       carry = behind;
     }
@@ -642,7 +655,7 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
   };
   request(row);
 #pragma unroll
-  for (int v = 0; v < 4; ++v) A[v] = v < n ? p.A[c0 + v] : 0.0f;
+  for (int v = 0; v < 4; ++v) A[v] = v < n ? rate(p.A[c0 + v]) : 0.0f;
   const long slot = p.at ? slot_of(row) : row;
   const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (slot < 0 || slot >= p.slots) return Four<BF>::store(p.y, (long)row * p.C + c0, n, none);

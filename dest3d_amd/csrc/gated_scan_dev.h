@@ -29,13 +29,12 @@ struct GScanP {
 constexpr int GS_TICKET = 32, GS_LOOK = 4;
 
 // What a tile tells the ones behind it of a channel, in one access of 8 bytes, so that nothing needs an order of its own: the map of its tokens,
-// H below P, or the state behind it, H below the bits of -0 (P is never negative: a tile with a cut knows the state behind it), or, all bits set,
-// nothing yet.
+// H below P, or the state behind it, H below the bits of -0 (P is a number, never negative: a tile with a cut knows the state behind it), or, all
+// bits set, nothing yet.
 constexpr unsigned GS_STATE = 0x80000000u, GS_NOTHING = 0xffffffffu;
 __device__ __forceinline__ void tell(unsigned long long* at, float H, unsigned high) {
   __hip_atomic_store(at, (unsigned long long)high << 32 | __float_as_uint(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ unsigned map_bits(float P) { return P != P ? 0x7fc00000u : __float_as_uint(P); }
 
 struct GStepP {
   int rows, C, ncb;
@@ -117,6 +116,9 @@ struct Piece {
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ex2(-LOG2E * x)); }
+// Growth that four tokens of a segment multiply within fp32 (exp(80) = 6e34); beyond it a channel is NaN, whichever form a call takes
+constexpr float GS_MOST = 20.0f;
+__device__ __forceinline__ float rate(float A) { return A > GS_MOST ? __builtin_nanf("") : A; }
 // a = exp(l) and beta = sqrt(1 - a^2).  Up to |l| = 1/4, -expm1(l) as its series: what is left out is below 2^-24 of it (l^6 / 7! = 4.8e-8).
 // NEAR: no l is beyond that (the same values, without the other form's exponential)
 constexpr float GS_NEAR = 0.25f;

@@ -730,7 +730,8 @@ int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t 
  * A state of one number for each channel, decayed by a gate and fed by the input:
  *   r = sigmoid(gate), l = A r, a = exp(l), beta = sqrt(1 - a^2) (ISSM_GS_NORMALIZE; else 1), u = sigmoid(in_gate) x (x without in_gate)
  *   h_t = a_t h_{t-1} + beta_t u_t,   y = h,   last = the state behind the last token
- * A <= 0 with ISSM_GS_NORMALIZE (a positive entry gives NaN there).  x, gate, in_gate, dy (B, L, C) in `dtype`, channels contiguous, element
+ * A <= 0 with ISSM_GS_NORMALIZE (a positive entry gives NaN there).  Without it A <= 20 (a larger entry gives NaN in its channel): states may grow
+ * then, also by more than fp32 holds where they are small or 0 in front, and overflow where the states themselves leave fp32.  x, gate, in_gate, dy (B, L, C) in `dtype`, channels contiguous, element
  * strides of batch and token (0 repeats); y, dx, dgate, din_gate (B, L, C) contiguous in `dtype`; A, dA (C), h0, last, dlast, dh0 (B, C) fp32
  * contiguous.  seq_idx (B, L) int32 or NULL: every change of id from a token to the next cuts the recurrence, and no value passes, whatever it
  * is; h0 counts as id 0: it feeds a row whose first token has id 0 and no other.  ISSM_GS_REVERSE walks from the last token to the first ("first"

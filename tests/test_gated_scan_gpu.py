@@ -658,3 +658,87 @@ def test_widths_that_share_cache_lines(B, L, C, dtype, packed):
         assert torch.isfinite(v).all() and torch.equal(v, whole[k][..., :C]), k
     if L <= 130:
         check(got, ref(d, dy, dlast))
+
+
+# ------------------------------------------------------------------------------------------------ states that grow
+def grown(got, want, lim):
+    """Each channel by itself: the largest would hide the others."""
+    for k, w in want.items():
+        v = got[k].double().cpu()
+        assert v.shape == w.shape and torch.isfinite(w).all() and torch.isfinite(v).all(), k
+        over = tuple(range(w.dim() - 1))
+        off, size = torch.linalg.vector_norm(v - w, dim=over), torch.linalg.vector_norm(w, dim=over)
+        bar = (2 if k.startswith("d") else 1) * lim + (STEP if got[k].dtype == torch.bfloat16 else 0.0)
+        assert (off <= bar * size + 1e-30).all(), (k, (off / size.clamp_min(1e-300)).max().item(), bar)
+
+
+# One step's decay is off by 2^-24 times 6 l (the sigmoid's four roundings, the product's and the exponent's in base 2) and 2 (exponential and state), l = A r
+def step_error(l):
+    return (6 * l + 2) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C,packed,reverse", [(2, 300, 24, False, False), (2, 1500, 6, False, True), (1, 100, 5, False, False), (3, 1200, 7, True, False),
+                                                  (520, 200, 8, False, False), (520, 130, 7, True, True)])
+def test_states_that_grow_behind_zeros(B, L, C, packed, reverse, dtype):
+    """Positive A: inputs that are zero up to the last 20 tokens, gradients that are zero behind the first 20.  States and what they pass back are 0 over
+    many tiles whose decays' product is far beyond fp32."""
+    d, dy, dlast = make(B, L, C, dtype, seed=L, initial=False)
+    d["gate"] = (0.3 * d["gate"].float()).to(dtype)
+    d["A"] = 1.0 + 3.0 * torch.rand(C, generator=torch.Generator().manual_seed(L))
+    first, last = (slice(0, 20), slice(L - 20, L)) if not reverse else (slice(L - 20, L), slice(0, 20))
+    keep = torch.zeros(L, dtype=torch.bool)
+    keep[last] = True
+    d["x"][:, ~keep] = 0
+    keep[:] = False
+    keep[first] = True
+    dy[:, ~keep] = 0
+    if packed:   # (a cut among the zeros)
+        d["seq_idx"] = torch.zeros(B, L, dtype=torch.int32)
+        d["seq_idx"][:, L // 2:] = 1
+    kw = dict(normalize=False, reverse=reverse)
+    l = (d["A"] * torch.sigmoid(d["gate"].double())).max().item()
+    got, want = run(d, dy, dlast * 0, **kw), ref(d, dy, dlast * 0, **kw)
+    assert want["y"].abs().max() > 1e8 and want["dx"].abs().max() > 1e8
+    grown(got, want, 20 * step_error(l))
+
+
+@pytest.mark.parametrize("B,L,l,reverse", [(2, 130, 1.2, False), (2, 90, 1.7, False), (600, 90, 1.7, True), (1, 140, 1.1, True)])
+def test_small_states_that_grow(B, L, l, reverse):
+    """A state of 1e-36 that grows over a tile by more than fp32 holds, and a gradient that does, stay numbers."""
+    C = 8
+    d = dict(x=torch.zeros(B, L, C), gate=torch.zeros(B, L, C), A=torch.full((C,), 2 * l), in_gate=None, initial_states=torch.full((B, C), 1e-36), seq_idx=None)
+    dy, dlast = torch.zeros(B, L, C), torch.full((B, C), 1e-36)
+    kw = dict(normalize=False, reverse=reverse)
+    got, want = run(d, dy, dlast, **kw), ref(d, dy, dlast, **kw)
+    grown({k: got[k] for k in want if k != "dx"}, {k: want[k] for k in want if k != "dx"}, L * step_error(l))
+    grown(dict(dx=got["dx"]), dict(dx=want["dx"]), L * step_error(l))
+
+
+def test_growth_within_a_window():
+    """Growth over 30 tokens among ones that change nothing (empty gates): all gradients, A's among them."""
+    d, dy, dlast = make(2, 400, 12, torch.float32)
+    d["A"] = 1.0 + 2.0 * torch.rand(12, generator=torch.Generator().manual_seed(4))
+    keep = torch.zeros(400, dtype=torch.bool)
+    keep[150:180] = True
+    d["gate"][:, ~keep] = -200.0
+    d["gate"][:, keep] *= 0.3
+    l = (d["A"] * torch.sigmoid(d["gate"].double())).max().item()
+    got, want = run(d, dy, dlast, normalize=False), ref(d, dy, dlast, normalize=False)
+    # (30 steps that grow; 370 sums in which all terms stay, 2^-24 each)
+    grown(got, want, 30 * step_error(l) + 370 * 2.0 ** -24)
+
+
+def test_growth_beyond_what_is_computed():
+    """A channel with A above 20 is NaN, in sequences and token by token; its neighbours are as they were."""
+    from dest3d_amd import gated_scan, gated_scan_step
+    for B, L in ((2, 300), (2, 1)):
+        d, _, _ = make(B, L, 6, torch.float32)
+        g = {k: None if v is None else v.cuda() for k, v in d.items()}
+        want = gated_scan(**g, normalize=False)
+        g["A"][3] = 20.5
+        got = gated_scan(**g, normalize=False)
+        assert torch.isnan(got[..., 3]).all() and torch.equal(got[..., [0, 1, 2, 4, 5]], want[..., [0, 1, 2, 4, 5]])
+    state = g["initial_states"].clone()
+    gated_scan_step(g["x"][:, 0], g["gate"][:, 0], g["A"], state, in_gate=g["in_gate"][:, 0], normalize=False)
+    assert torch.isnan(state[:, 3]).all() and torch.isfinite(state[:, [0, 1, 2, 4, 5]]).all()
