@@ -583,7 +583,8 @@ __global__ __launch_bounds__(GS_THREADS, BF && SHARED ? 6 : 2) void k_gscan_bwd(
           dx[v] = du * sg[s][v];
           di[v] = dx[v] * xv * (1.0f - sg[s][v]);
           dg[v] = dl * l * (1.0f - r[s][v]);
-          sum[v] = fmaf(dl, r[s][v], sum[v]);
+          // (an empty gate, as behind the end, gives nothing to any sum: the state may be infinite there, or a last state's gradient)
+          sum[v] = r[s][v] == 0.0f ? sum[v] : fmaf(dl, r[s][v], sum[v]);
         }
         if (p.dx) to_x.store(s, dx);
         if (p.dg) to_g.store(s, dg);

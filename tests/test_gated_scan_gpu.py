@@ -742,3 +742,26 @@ def test_growth_beyond_what_is_computed():
     state = g["initial_states"].clone()
     gated_scan_step(g["x"][:, 0], g["gate"][:, 0], g["A"], state, in_gate=g["in_gate"][:, 0], normalize=False)
     assert torch.isnan(state[:, 3]).all() and torch.isfinite(state[:, [0, 1, 2, 4, 5]]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C", [(2, 56, 8), (2, 57, 8), (3, 100, 7), (2, 225, 64), (1, 1, 4), (520, 57, 8)])
+def test_no_number_at_the_last_token(B, L, C, dtype):
+    """An infinite state behind the row, or an infinite gradient of a last state that a cut keeps from the row: the gradient of A is that of the tokens
+    in front, bit for bit, however far the row's last tile reaches."""
+    d, dy, dlast = make(B, L, C, dtype)
+    clean = run(d, dy, dlast, normalize=False)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        e = dict(d, x=d["x"].clone())
+        e["x"][:, -1] = bad
+        got = run(e, dy, dlast, normalize=False)
+        assert not torch.isfinite(got["last"]).any() and torch.equal(got["dA"], clean["dA"]) and torch.equal(got["dx"], clean["dx"])
+        cut = dict(d, seq_idx=torch.zeros(B, L, dtype=torch.int32))
+        cut["seq_idx"][:, -1] = 1
+        want = run(cut, dy, dlast, normalize=False)
+        got = run(cut, dy, torch.full_like(dlast, bad), normalize=False)
+        assert torch.isfinite(got["dA"]).all()
+        for k in ("dA", "dinitial_states"):
+            assert torch.equal(got[k], want[k]), k
+        for k in ("dx", "dgate", "din_gate"):
+            assert torch.equal(got[k][:, :-1], want[k][:, :-1]), k
