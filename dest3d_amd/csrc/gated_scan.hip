@@ -727,9 +727,9 @@ template <bool BF, int V, int IG, int NRM, bool SHARED, bool BUF>
 static void launch_packed(const GScanP& p, bool back, int blocks, hipStream_t st) {
   p.ids ? launch_one<BF, V, IG, NRM, true, SHARED, BUF>(p, back, blocks, st) : launch_one<BF, V, IG, NRM, false, SHARED, BUF>(p, back, blocks, st);
 }
-template <bool BF, int IG, int NRM>
+template <bool BF, int V, int IG, int NRM, bool BUF>
 static void launch_shared(const GScanP& p, bool back, int blocks, hipStream_t st) {
-  p.words ? launch_packed<BF, 4, IG, NRM, true, true>(p, back, blocks, st) : launch_packed<BF, 4, IG, NRM, false, true>(p, back, blocks, st);
+  p.words ? launch_packed<BF, V, IG, NRM, true, BUF>(p, back, blocks, st) : launch_packed<BF, V, IG, NRM, false, BUF>(p, back, blocks, st);
 }
 // Rows that buffers take: whole dwords, a tile's rows (and one more) within 2^31 bytes
 static bool behind_buffers(const GScanP& p, bool bf, bool back) {
@@ -741,13 +741,13 @@ static bool behind_buffers(const GScanP& p, bool bf, bool back) {
 }
 template <bool BF>
 static void launch_form(const GScanP& p, bool buffers, bool back, int blocks, hipStream_t st) {
-  if (!buffers) {   // (one form for both ways of taking the tiles: a workgroup that takes all of a row's finds its own states)
-    if (p.C >= 4) launch_packed<BF, 4, 2, 2, true, false>(p, back, blocks, st);
-    else launch_packed<BF, 1, 2, 2, true, false>(p, back, blocks, st);
+  if (!buffers) {
+    if (p.C >= 4) launch_shared<BF, 4, 2, 2, false>(p, back, blocks, st);
+    else launch_shared<BF, 1, 2, 2, false>(p, back, blocks, st);
   } else if (p.i) {
-    p.nrm ? launch_shared<BF, 1, 1>(p, back, blocks, st) : launch_shared<BF, 1, 0>(p, back, blocks, st);
+    p.nrm ? launch_shared<BF, 4, 1, 1, true>(p, back, blocks, st) : launch_shared<BF, 4, 1, 0, true>(p, back, blocks, st);
   } else {
-    p.nrm ? launch_shared<BF, 0, 1>(p, back, blocks, st) : launch_shared<BF, 0, 0>(p, back, blocks, st);
+    p.nrm ? launch_shared<BF, 4, 0, 1, true>(p, back, blocks, st) : launch_shared<BF, 4, 0, 0, true>(p, back, blocks, st);
   }
 }
 
@@ -758,33 +758,43 @@ constexpr int GS_WG = 2, GS_WG_BACK = 3, GS_ROWS_WALKED = 2 * NCU;
 static int sharing(int rows, int tiles, bool back) {
   return rows >= GS_ROWS_WALKED ? 1 : max(1, min(tiles, ((back ? GS_WG_BACK : GS_WG) * NCU + rows - 1) / rows));
 }
-// A call's workspace: partial sums of dA, then the tickets and what the tiles tell, in whole 16 bytes each; for the finest tiles it may take
-static size_t part_bytes(int B, int L, int C) { return ((size_t)B * gscan_tiles(L, GS_S_BACK) * C * 4 + 255) & ~(size_t)255; }
-static size_t ticket_bytes(int B, int C) { return (size_t)B * gscan_blocks(C) * GS_TICKET * 4; }
-static size_t word_bytes(int B, int L, int C, int S) { return (size_t)B * gscan_blocks(C) * (gscan_tiles(L, S) + GS_LOOK) * 64 * 8; }
-size_t gscan_workspace(int B, int L, int C, bool back) {
-  return (back ? part_bytes(B, L, C) : 0) + ticket_bytes(B, C) + word_bytes(B, L, C, back ? GS_S_BACK : GS_S_SHARED);
+// A call's tiles of a row, how many workgroups share it, and its workspace: partial sums of dA, a row for each tile where tiles are shared and for
+// each row where it is walked, then (shared) the tickets and what the tiles tell, in whole 16 bytes each.  All of it goes by sizes alone.
+struct GScanPlan {
+  int share, nk;
+  size_t part, tickets, words;
+  GScanPlan(int B, int L, int C, bool back, bool dA) {
+    const int ncb = gscan_blocks(C), rows = B * ncb, S = back ? GS_S_BACK : GS_S_SHARED;
+    share = sharing(rows, gscan_tiles(L, S), back);
+    nk = gscan_tiles(L, share > 1 || back ? S : GS_S_WALKED);
+    part = dA ? ((size_t)B * (share > 1 ? nk : 1) * C * 4 + 255) & ~(size_t)255 : 0;
+    tickets = share > 1 ? (size_t)rows * GS_TICKET * 4 : 0;
+    words = share > 1 ? (size_t)rows * (nk + GS_LOOK) * 64 * 8 : 0;
+  }
+};
+size_t gscan_workspace(int B, int L, int C, bool back, bool dA) {
+  const GScanPlan plan(B, L, C, back, back && dA);
+  return plan.part + plan.tickets + plan.words;
 }
 
 int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st) {
+  const GScanPlan plan(p.B, p.L, p.C, back, back && p.dA);
+  const bool shared = plan.share > 1;
   p.ncb = gscan_blocks(p.C);
   p.nb = gscan_tiles(p.L, GS_S_BACK);
-  const int rows = p.B * p.ncb, S = back ? GS_S_BACK : GS_S_SHARED, share = sharing(rows, gscan_tiles(p.L, S), back);
-  const bool buffers = behind_buffers(p, bf, back), shared = share > 1 || !buffers;
-  p.nk = shared || back ? gscan_tiles(p.L, S) : gscan_tiles(p.L, GS_S_WALKED);
-  p.lines = (p.C * (bf ? 2L : 4L)) % 128 != 0 && (share == 1 || 2 * p.nk >= 3 * share);
+  p.nk = plan.nk;
+  p.lines = (p.C * (bf ? 2L : 4L)) % 128 != 0 && (!shared || 2 * p.nk >= 3 * plan.share);
   char* ws = (char*)workspace;
-  if (back) {
-    p.part = p.dA ? (float*)ws : nullptr;
-    ws += part_bytes(p.B, p.L, p.C);
-  }
+  if (plan.part) p.part = (float*)ws;
   if (shared) {
+    ws += plan.part;
     p.tickets = (unsigned*)ws;
-    p.words = (unsigned long long*)(ws + ticket_bytes(p.B, p.C));
-    const long n = (long)((ticket_bytes(p.B, p.C) + word_bytes(p.B, p.L, p.C, S)) / 16);
+    p.words = (unsigned long long*)(ws + plan.tickets);
+    const long n = (long)((plan.tickets + plan.words) / 16);
     k_gscan_clear<<<(int)min((n + 1023) / 1024, 1024L), 256, 0, st>>>((uint4*)ws, n);
   }
-  bf ? launch_form<true>(p, buffers, back, rows * share, st) : launch_form<false>(p, buffers, back, rows * share, st);
+  const int blocks = p.B * p.ncb * plan.share;
+  bf ? launch_form<true>(p, behind_buffers(p, bf, back), back, blocks, st) : launch_form<false>(p, behind_buffers(p, bf, back), back, blocks, st);
   if (p.part) k_gscan_sum<<<(p.C + 15) / 16, 1024, 0, st>>>(p.part, shared ? p.B * p.nk : p.B, p.C, p.dA);
   return (int)hipGetLastError();
 }

@@ -88,7 +88,7 @@ int launch_dwconv_bwd(const DwConvP& p, hipStream_t st);
 int pgen_bwd_blocks(long tokens);
 int launch_pgen_fwd(const PGenP& p, hipStream_t st);
 int launch_pgen_bwd(const PGenP& p, hipStream_t st);
-size_t gscan_workspace(int B, int L, int C, bool back);
+size_t gscan_workspace(int B, int L, int C, bool back, bool dA);
 int launch_gscan(GScanP p, bool bf, bool back, void* workspace, hipStream_t st);
 int launch_gscan_step(GStepP p, bool bf, bool nrm, hipStream_t st);
 int launch_rotary(RotP p, bool bf, bool inter, bool norm, hipStream_t st);
@@ -1452,14 +1452,14 @@ int issm_gated_scan_workspace_bytes(const issm_gated_scan_args* a, int32_t backw
   int rc = gscan_sizes(a);
   if (rc) return rc;
   if (!out) return fail(ISSM_E_NULL, "out is NULL");
-  *out = gscan_workspace(a->batch, a->seqlen, a->channels, backward);
+  *out = gscan_workspace(a->batch, a->seqlen, a->channels, backward, true);
   return ISSM_OK;
 }
 
 static int gscan_call(const issm_gated_scan_args* a, bool back) {
-  size_t need = 0;
-  int rc = issm_gated_scan_workspace_bytes(a, back, &need);
+  int rc = gscan_sizes(a);
   if (rc) return rc;
+  const size_t need = gscan_workspace(a->batch, a->seqlen, a->channels, back, a->dA);
   if (!a->x || !a->gate || !a->A) return fail(ISSM_E_NULL, "gated_scan: x/gate/A is NULL");
   if (!back && !a->y) return fail(ISSM_E_NULL, "gated_scan: y is NULL");
   if (back && !a->saved) return fail(ISSM_E_NULL, "gated_scan bwd: saved is NULL");

@@ -737,7 +737,7 @@ int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t 
  * is; h0 counts as id 0: it feeds a row whose first token has id 0 and no other.  ISSM_GS_REVERSE walks from the last token to the first ("first"
  * and "last" above in the walk's order).  States, decays and sums are fp32; results are bit-reproducible.
  * saved: issm_gated_scan_saved_bytes, the states that the backward starts its tiles from; NULL in a forward that none follows.  workspace:
- * issm_gated_scan_workspace_bytes (may be 0).  Backward: dy, dlast NULL = zero, dx, dgate, din_gate, dA, dh0 NULL = not wanted; where beta = 0 (nothing
+ * issm_gated_scan_workspace_bytes (may be 0; a backward without dA may need less).  Backward: dy, dlast NULL = zero, dx, dgate, din_gate, dA, dh0 NULL = not wanted; where beta = 0 (nothing
  * decays) it has no derivative: its part of dgate and dA is taken as 0.  A token whose gate is empty in fp32 gives nothing to dA. */
 #define ISSM_GS_NORMALIZE 1u
 #define ISSM_GS_REVERSE 2u

@@ -765,3 +765,39 @@ def test_no_number_at_the_last_token(B, L, C, dtype):
             assert torch.equal(got[k], want[k]), k
         for k in ("dx", "dgate", "din_gate"):
             assert torch.equal(got[k][:, :-1], want[k][:, :-1]), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C,packed", [(520, 130, 8, 0), (300, 113, 72, 2), (3, 100, 8, 0), (600, 1, 8, 0)])
+def test_walked_rows_by_all_addresses(B, L, C, packed, dtype):
+    """Rows that one workgroup walks, at odd places: what aligned ones give, bit for bit."""
+    d, dy, dlast = make(B, L, C, dtype, packed=packed)
+    want = run(d, dy, dlast)
+    wide = torch.empty(B * L * (C + 3) + 1, dtype=dtype, device="cuda")
+    odd = wide.as_strided((B, L, C), (L * (C + 3), C + 3, 1), 1)
+    odd.copy_(d["x"])
+    got = run(dict(d, x=odd), dy, dlast)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_memory_of_many_short_rows():
+    """A call of single tokens takes its results, and in the backward a row of partial sums for each row, beside its inputs."""
+    from dest3d_amd import gated_scan
+    B, C = 4096, 2048
+    for width in (C, C - 1):
+        x = torch.randn(B, 1, width, device="cuda", dtype=torch.bfloat16)
+        A = torch.full((width,), -1.0, device="cuda")
+        size = x.numel() * 2
+        gated_scan(x, x, A)
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = gated_scan(x, x, A)
+        assert torch.cuda.max_memory_allocated() - start <= size + (1 << 21)
+        leaves = [x.detach().requires_grad_(), x.detach().clone().requires_grad_(), A.detach().requires_grad_()]
+        y = gated_scan(*leaves)
+        start = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        torch.autograd.grad(y, leaves, x)
+        assert torch.cuda.max_memory_allocated() - start <= 4 * size + (1 << 21)   # two gradients in bf16, sums in fp32
+        torch.autograd.grad(gated_scan(*leaves[:2], A), leaves[:2], x)

@@ -172,3 +172,23 @@ def test_oracle():
         one, two = (slice(0, 6, 2), slice(1, 6, 2)) if inter else (slice(0, 3), slice(3, 6))
         z = torch.complex(v[..., one], v[..., two]) * torch.polar(torch.ones_like(angle), angle)[None, :, None]
         torch.testing.assert_close(torch.complex(w[..., one], w[..., two]), z)
+
+
+@pytest.mark.parametrize("batch,seqlen,channels", [(8192, 1, 4096), (65535, 1, 4032), (600, 4096, 64), (513, 100000, 7), (3, 100, 64), (1, 1, 1)])
+def test_workspace_of_walked_rows(lib, batch, seqlen, channels):
+    """Rows that a workgroup walks ask for nothing forward, and backward for a row of dA's sums each; shared ones for less than the data."""
+    a, need = _scan(lib, batch=batch, seqlen=seqlen, channels=channels), C.c_size_t()
+    assert lib.issm_gated_scan_workspace_bytes(C.byref(a), 0, C.byref(need)) == 0 and need.value == 0
+    assert lib.issm_gated_scan_workspace_bytes(C.byref(a), 1, C.byref(need)) == 0
+    if (batch, seqlen) != (3, 100):   # (one tile forward, two backward: shared)
+        assert batch * channels * 4 <= need.value < batch * channels * 4 + 256
+
+
+@pytest.mark.parametrize("batch,seqlen,channels", [(1, 131072, 2048), (8, 4096, 2048), (2, 1000, 288), (511, 113, 64)])
+def test_workspace_of_shared_rows(lib, batch, seqlen, channels):
+    """8 bytes a channel for 112 tokens, backward for 56, and there 4 for dA's sums; beside them what five tiles take, and the tickets."""
+    a, need, size = _scan(lib, batch=batch, seqlen=seqlen, channels=channels), C.c_size_t(), batch * seqlen * channels
+    rows = batch * -(-channels // 64)
+    for back, share in ((0, 8 / 112), (1, 12 / 56)):
+        assert lib.issm_gated_scan_workspace_bytes(C.byref(a), back, C.byref(need)) == 0
+        assert 0 < need.value < share * size * 1.15 + rows * (128 + 5 * 512 + 256)   # (288 channels take the words of 320)
