@@ -1437,7 +1437,8 @@ struct GatedScanFn : public Function<GatedScanFn> {
     const GatedScan s = GatedScan::make(x, gate, A, in_gate, h0, seq, normalize, reverse);
     GatedScan::Out o = s.forward(want_last, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({s.x, s.gate, s.A, s.in_gate, s.h0, s.seq, o.saved});   // (the inputs themselves where the kernels read those)
+    // (the inputs themselves where the kernels read those; the initial states are in `saved`, and may change)
+    ctx->save_for_backward({s.x, s.gate, s.A, s.in_gate, s.seq, o.saved});
     auto r = c10::make_intrusive<Record>();
     const Tensor* in[NIN] = {&x, &gate, &A, &in_gate, &h0};
     for (int i = 0; i < NIN; ++i) {
@@ -1462,8 +1463,7 @@ struct GatedScanFn : public Function<GatedScanFn> {
     s.gate = v[1];
     s.A = v[2];
     s.in_gate = v[3];
-    s.h0 = v[4];
-    s.seq = v[5];
+    s.seq = v[4];
     s.normalize = in->normalize;
     s.reverse = in->reverse;
     const c10::DeviceGuard guard(s.x.device());
@@ -1478,7 +1478,7 @@ struct GatedScanFn : public Function<GatedScanFn> {
       if (g[4].defined()) dlast.defined() ? g[4].copy_(dlast) : g[4].zero_();
     } else {
       issm_gated_scan_args a = s.args();
-      a.saved = data(v[6]);
+      a.saved = data(v[5]);
       if (dy.defined()) {
         a.dy = data(dy);
         a.dy_stride[0] = dy.stride(0);

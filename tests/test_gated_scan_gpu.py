@@ -801,3 +801,17 @@ def test_memory_of_many_short_rows():
         torch.autograd.grad(y, leaves, x)
         assert torch.cuda.max_memory_allocated() - start <= 4 * size + (1 << 21)   # two gradients in bf16, sums in fp32
         torch.autograd.grad(gated_scan(*leaves[:2], A), leaves[:2], x)
+
+
+def test_initial_states_may_change_before_the_backward():
+    """The backward does not read them: a buffer of states that the next call's take over is no error, and the gradients are the same."""
+    from dest3d_amd import gated_scan
+    for L in (90, 700, 0):
+        d, dy, dlast = make(2, L, 24, torch.float32)
+        g = {k: None if v is None else v.cuda() for k, v in d.items()}
+        leaves = [g[k].requires_grad_() for k in ("x", "gate", "A", "in_gate")]
+        want = torch.autograd.grad(gated_scan(**g, return_final_states=True), leaves, (dy.cuda(), dlast.cuda()), allow_unused=L == 0)
+        y, last = gated_scan(**g, return_final_states=True)
+        g["initial_states"].copy_(last.detach() + 1.0)
+        got = torch.autograd.grad((y, last), leaves, (dy.cuda(), dlast.cuda()), allow_unused=L == 0)
+        assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
