@@ -6,7 +6,6 @@
 // kernels (and, for the layer's four projections, in the tensor library's matrix products).
 #include <Python.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/SavedTensorHooks.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
@@ -1539,10 +1538,18 @@ std::vector<Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Tensor
   return out;
 }
 
-// (of two tensors with gaps in one allocation it cannot be told)
-bool shares_memory(const Tensor& a, const Tensor& b) {
-  const at::MemOverlapStatus s = at::get_overlap_status(a, b);
-  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+// Whether one of an operand's rows, as the kernel reads them, has a byte of one of the state's slots: by addresses, gaps between rows and slots included
+bool in_slots(const Tensor& t, const Tensor& state) {
+  if (!t.defined() || t.numel() == 0 || state.numel() == 0) return false;
+  const int64_t rows = t.dim() > 1 ? t.size(0) : 1, step = rows > 1 ? t.stride(0) * (int64_t)t.element_size() : 0, row = t.size(-1) * (int64_t)t.element_size();
+  const int64_t slots = state.size(0), slot = state.size(1) * (int64_t)sizeof(float), apart = slots > 1 ? state.stride(0) * (int64_t)sizeof(float) : slot;
+  int64_t at = (int64_t)((intptr_t)t.data_ptr() - (intptr_t)state.data_ptr());
+  if (at + (rows - 1) * step + row <= 0 || at >= (slots - 1) * apart + slot) return false;
+  for (int64_t r = 0; r < rows; ++r, at += step) {
+    const int64_t end = at + row;   // the last slot that starts in front of it
+    if (end > 0 && std::min((end - 1) / apart, slots - 1) * apart + slot > at) return true;
+  }
+  return false;
 }
 
 Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, const Tensor& state, const MaybeTensor& in_gate_,
@@ -1564,8 +1571,6 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, con
   const int64_t rows = x.size(0), C = x.size(1), slots = state.size(0);
   require((C <= 1 || state.stride(1) == 1) && (slots <= 1 || state.stride(0) >= C) && !state.is_neg(),
           "state must have contiguous channels and slots that do not overlap (it is updated in place)");
-  for (const Tensor* t : {&x, &gate, &A, &in_gate})
-    require(!t->defined() || !shares_memory(*t, state), "state must share no memory with the other operands (it is updated in place)");
   if (at.defined()) {
     require_shape(at.dim() == 1 && at.size(0) == rows, "state_indices", "(rows,)", at);
     require_type(is_index(at), "state_indices", "int32 or int64", at);
@@ -1575,11 +1580,13 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& A, con
   require_shape(rows <= INT32_MAX && C <= INT32_MAX, "x", "of fewer than 2^31 entries a dimension", x);
   if (recorded({&x, &gate, &A, &state, &in_gate}))
     raise_py(PyExc_RuntimeError, "gated_scan_step has no backward: call it under torch.no_grad(), or gated_scan");
-  py::gil_scoped_release release;
   const c10::DeviceGuard guard(x.device());
   const at::ScalarType io = common_type({&x, &gate, &in_gate});
   const Tensor xk = kernel_operand(x, io), gk = kernel_operand(gate, io), ik = kernel_operand(in_gate, io), Ak = f32c(in_memory(A)),
                ak = at.defined() ? at.contiguous() : at;
+  for (const Tensor* t : {&xk, &gk, &ik, &Ak, &ak})
+    require(!in_slots(*t, state), "state must share no memory with the other operands (it is updated in place)");
+  py::gil_scoped_release release;
   const Tensor y = fresh(x.sizes(), x, io);
   if (x.numel() == 0) return cast(y, x.scalar_type());
   if (slots == 0) return cast(y.zero_(), x.scalar_type());

@@ -815,3 +815,32 @@ def test_initial_states_may_change_before_the_backward():
         g["initial_states"].copy_(last.detach() + 1.0)
         got = torch.autograd.grad((y, last), leaves, (dy.cuda(), dlast.cuda()), allow_unused=L == 0)
         assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+
+
+def test_step_refuses_its_state_as_an_input_in_a_pool_with_gaps():
+    """Slots that lie apart: an input that has a number of one of them is refused; what lies beside them, between them or was copied is not."""
+    from dest3d_amd import gated_scan_step
+    C, A, at = 8, torch.full((8,), -1.0, device="cuda"), torch.tensor([2, 0, 3, 1], device="cuda")
+    wide = torch.randn(9, 24, device="cuda")
+    before = wide.clone()
+    state, x = wide[:4, 8:16], torch.randn(4, C, device="cuda")
+    for bad in (wide[:4, 8:16], wide[:4, 3:11], wide[:4, 15:23], wide[3:7, 8:16], wide[:8:2, 8:16], wide[3].view(1, 24)[:, 8:16].expand(4, C),
+                wide.flatten()[13:61].view(4, 12)[:, 3:11]):   # (rows 12 apart, at 16, 28, 40, 52: the second and the fourth)
+        for kw in (dict(x=bad), dict(gate=bad), dict(in_gate=bad)):
+            with pytest.raises(AssertionError, match="share no memory"):
+                gated_scan_step(**{**dict(x=x, gate=x, A=A, state=state, state_indices=at), **kw})
+    with pytest.raises(AssertionError, match="share no memory"):
+        gated_scan_step(x, x, wide[3, 12:20], state, state_indices=at)
+    with pytest.raises(AssertionError, match="share no memory"):
+        gated_scan_step(x, x, A, state, state_indices=wide.view(torch.int32)[1, 10:14])
+    assert torch.equal(wide, before)
+    for good in (wide[:4, :8], wide[:4, 16:], wide[4:8, 8:16], wide[5:9, 8:16], wide[4:8, 8:16].bfloat16(), torch.as_strided(wide, (4, C), (48, 1), 16)):
+        copy = wide[:4, 8:16].clone()
+        want = gated_scan_step(good.clone(), x, A, copy, in_gate=good.clone(), state_indices=at)
+        got = gated_scan_step(good, x, A, state, in_gate=good, state_indices=at)
+        assert torch.equal(got, want) and torch.equal(state, copy)
+    # channels apart: the kernel reads a copy, made before a state changes
+    square = torch.randn(C, C, device="cuda")
+    copy = square.clone()
+    want = gated_scan_step(square.t().clone(), square.t().clone(), A, copy)
+    assert torch.equal(gated_scan_step(square.t(), square.t(), A, square), want) and torch.equal(square, copy)
