@@ -211,7 +211,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int lpr) {
 template <bool BF, int V, int NI, bool INTER, bool NORM, int NB, bool MANY>
 __global__ __launch_bounds__(256) void k_rotary(RotP p) {
   const int lane = threadIdx.x & 63, li = lane & (p.lpr - 1), sub = lane / p.lpr, tokens = 64 / p.lpr / p.group;   // tokens at a time
-  unsigned unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  unsigned unit = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned part = p.by_parts(unit);
   const int heads = p.H[0] + p.H[1], h0 = (int)part * p.heads_each * p.group + sub % p.group, mine = sub / p.group;
   const long t0 = (long)unit * (MANY ? NB : 1) * tokens + mine;
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(1024) void k_rotary_dw(RotP p) {
 // Units of work: a wave each, as few heads a wave as it takes to have WAVES of them
 constexpr long WAVES = 4096;
 template <bool BF, int V, int NI, bool INTER, bool NORM>
-static bool launch_rows(RotP& p, hipStream_t st) {
+static void launch_rows(RotP& p, hipStream_t st) {
   constexpr int NB = NI > 1 || !NORM ? 1 : 2;   // (16384 tokens of 32 and 8 heads of 128, bf16, with the norm, 1, 2, 4: 73.6, 68.5, 95.0 us; 65536 of 16
                                                 // and 4, without, 1 and 2: 129 and 136)
   const int rows = 64 / p.lpr, heads = p.H[0] + p.H[1];
@@ -400,13 +400,16 @@ static bool launch_rows(RotP& p, hipStream_t st) {
   p.by_parts = div_by((unsigned)parts);
   const bool many = p.heads_each == 1 && units * parts >= 2 * WAVES;   // (waves enough with several tokens each)
   const long waves = (many ? (units + NB - 1) / NB : units) * parts, blocks = (waves + 3) / 4;
-  if (blocks >= 1L << 24) return false;   // (a launch has fewer than 2^32 threads)
-  if (many) k_rotary<BF, V, NI, INTER, NORM, NB, true><<<(unsigned)blocks, 256, 0, st>>>(p);
-  else k_rotary<BF, V, NI, INTER, NORM, NB, false><<<(unsigned)blocks, 256, 0, st>>>(p);
-  return true;
+  constexpr long MOST = (1L << 24) - 1;   // (a launch has fewer than 2^32 threads: 2^26 rows of 33 pairs go in two)
+  for (long b = 0; b < blocks; b += MOST) {
+    p.first = (unsigned)b;
+    const unsigned n = (unsigned)min(blocks - b, MOST);
+    if (many) k_rotary<BF, V, NI, INTER, NORM, NB, true><<<n, 256, 0, st>>>(p);
+    else k_rotary<BF, V, NI, INTER, NORM, NB, false><<<n, 256, 0, st>>>(p);
+  }
 }
 template <bool BF, int V, int NI, bool INTER>
-static bool launch_norm_bwd(RotP& p, hipStream_t st) {
+static void launch_norm_bwd(RotP& p, hipStream_t st) {
   constexpr int NB = 1;   // (4096 x 4 tokens of 16 and 4 heads of 128, bf16, 1 and 2: 46.6 and 52.9 us)
   const int rows = 64 / p.lpr;
   bool many = true;
@@ -418,13 +421,12 @@ static bool launch_norm_bwd(RotP& p, hipStream_t st) {
   const unsigned blocks = p.blocks[0] + p.blocks[1], bytes = 4 * p.D * sizeof(float);
   if (many) k_rotary_norm_bwd<BF, V, NI, INTER, NB, true><<<blocks, 256, bytes, st>>>(p);
   else k_rotary_norm_bwd<BF, V, NI, INTER, NB, false><<<blocks, 256, bytes, st>>>(p);
-  return true;
 }
 
 // V: the widest that both parts of a head, turned and not, are whole multiples of, if 64 lanes hold a row; up to 16 bytes an access forward (16384 tokens
 // of 32 and 8 heads of 128, bf16, 8 and 4: 68.5 and 86.7 us), 4 backwards, where wider ones leave too few waves (46.8 and 43.7 us, heads of 64 29.6 and 25.9)
 template <bool BF, bool INTER>
-static bool launch_widths(RotP& p, bool norm, bool back, hipStream_t st) {
+static void launch_widths(RotP& p, bool norm, bool back, hipStream_t st) {
   const int half = p.R / 2, rest = p.D - p.R;
   int V = 1;
   for (int v = BF && !back ? 8 : 4; v > 1; v >>= 1)
@@ -455,10 +457,9 @@ static void divisors(RotP& p) {
 
 int launch_rotary(RotP p, bool bf, bool inter, bool norm, hipStream_t st) {
   divisors(p);
-  bool ok;
-  if (bf) ok = inter ? launch_widths<true, true>(p, norm, false, st) : launch_widths<true, false>(p, norm, false, st);
-  else ok = inter ? launch_widths<false, true>(p, norm, false, st) : launch_widths<false, false>(p, norm, false, st);
-  return ok ? (int)hipGetLastError() : (int)hipErrorInvalidConfiguration;
+  if (bf) inter ? launch_widths<true, true>(p, norm, false, st) : launch_widths<true, false>(p, norm, false, st);
+  else inter ? launch_widths<false, true>(p, norm, false, st) : launch_widths<false, false>(p, norm, false, st);
+  return (int)hipGetLastError();
 }
 
 int launch_rotary_norm_bwd(RotP p, bool bf, bool inter, hipStream_t st) {

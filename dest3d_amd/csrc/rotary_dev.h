@@ -9,6 +9,7 @@ constexpr int ROT_MAX_D = 1024;
 struct RotP {
   int L, D, R, tokens, H[2];      // tokens = B L; H: heads of the two sides, 0 of one that is absent
   int lpr, pairs, blocks[2];
+  unsigned first;                 // the launch's first workgroup, where there are more than one launches
   int group, heads_each, groups[2];   // heads of a token that a wave has at a time, times how often; and of a side, backwards
   Div by_parts, by_L;
   float inv_D;

@@ -390,3 +390,18 @@ def test_table_without_forward_derivative():
     q, tab = torch.zeros(1, 5, 2, 16, device="cuda"), table(5, 16).cuda()
     with fwAD.dual_level(), pytest.raises(AssertionError, match="no gradient"):
         rotary(q, None, fwAD.make_dual(tab, tab))
+
+
+@pytest.mark.parametrize("norm,tokens", [(False, 2 ** 26 + 2 ** 20 + 8), (True, 2 ** 27 + 8)])
+def test_more_waves_than_a_launch_has(norm, tokens):
+    """Heads of 66 features, a wave for each or for two of them: rows below 2^31, in more launches than one."""
+    from dest3d_amd import qk_norm_rotary, rotary
+    tab, w = table(8, 2).cuda(), torch.rand(66, device="cuda")
+    x = torch.randn(66, device="cuda").bfloat16()
+    call = (lambda q, **kw: qk_norm_rotary(q, None, w, None, tab, **kw)) if norm else (lambda q, **kw: rotary(q, None, tab, **kw))
+    want = call(x.expand(1, 8, 1, 66))[0, :, 0]
+    pos = torch.arange(8, device="cuda", dtype=torch.int32).repeat(tokens // 8)
+    y = call(x.expand(1, tokens, 1, 66), positions=pos)
+    assert not torch.equal(want[1], want[2])
+    for part in y.view(tokens // 8, 8, 66).split(2 ** 20):
+        assert (part == want).all()
