@@ -48,6 +48,7 @@ def rotary(q, k, table, positions=None, interleaved=False):
     """
     Argument:
         q: (batch, seqlen, heads, headdim), k: (batch, seqlen, kv_heads, headdim) or None; features contiguous, other strides as they are.
+            headdim up to 1024, batch * seqlen * (heads + kv_heads) below 2^31, heads + kv_heads up to 2^20.
             bfloat16 where both are, else computed in float32; each is returned in its own type
         table: (rows, rot) of rotary_table; the first rot <= headdim features of a head are turned, the others returned as they are
         positions: (batch, seqlen) or (seqlen,) int32 or int64, rows of the table, or None: 0, 1, ... along the sequence.  A position

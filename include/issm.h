@@ -738,7 +738,9 @@ int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t 
  * and "last" above in the walk's order).  States, decays and sums are fp32; results are bit-reproducible.
  * saved: issm_gated_scan_saved_bytes, the states that the backward starts its tiles from; NULL in a forward that none follows.  workspace:
  * issm_gated_scan_workspace_bytes (may be 0; a backward without dA may need less).  Backward: dy, dlast NULL = zero, dx, dgate, din_gate, dA, dh0 NULL = not wanted; where beta = 0 (nothing
- * decays) it has no derivative: its part of dgate and dA is taken as 0.  A token whose gate is empty in fp32 gives nothing to dA. */
+ * decays) it has no derivative: its part of dgate and dA is taken as 0.  A token whose gate is empty in fp32 gives nothing to dA.
+ * Sizes: seqlen <= 2^30, batch ceil(channels / 64) < 2^22, and that times ceil(seqlen / 28) < 2^24.  Where workgroups share a row they wait for each other's
+ * states; a wait that no state ends (the workspace overwritten from elsewhere) gives up after seconds with NaN in the states, not with an error. */
 #define ISSM_GS_NORMALIZE 1u
 #define ISSM_GS_REVERSE 2u
 typedef struct issm_gated_scan_args {
@@ -777,7 +779,8 @@ int issm_gated_scan_bwd(const issm_gated_scan_args* args);
 
 /* One token of `rows` sequences: x, gate, in_gate (rows, C) with element strides between rows, y (rows, C) contiguous, state (slots, C) fp32 with
  * state_stride >= C between slots, updated in place.  slots_of (rows) int32 or int64 (slots_64) names each row's slot, NULL: row r has slot r.  A row whose slot is
- * outside [0, slots) gives zeros and touches no state; rows of one slot are taken in their order, as tokens one behind the other. */
+ * outside [0, slots) gives zeros and touches no state; rows of one slot are taken in their order, as tokens one behind the other.  The state shares no
+ * memory with the others.  A as in issm_gated_scan_fwd; rows ceil(channels / 1024) < 2^23. */
 typedef struct issm_gated_scan_step_args {
   int32_t rows, channels;
   int64_t slots;
@@ -806,7 +809,8 @@ int issm_gated_scan_step(const issm_gated_scan_step_args* args);
  * (positions_64) with element strides (0 repeats) or NULL: a token's place in its sequence (seqlen <= table_rows then).  The turned features of
  * a position outside the table are NaN.  x, dy (B, L, H, D) in `dtype`, features contiguous, element strides of batch, token and head; y, dx
  * (B, L, H, D) contiguous.  w, dw (D) in weight_dtype.  ISSM_ROT_BACK turns the other way: issm_rotary's backward.  issm_rotary_norm_bwd's scratch:
- * issm_rotary_norm_bwd_bytes; dw[i] NULL = not wanted.  headdim <= 1024, rot even and >= 2, tokens times heads below 2^31. */
+ * issm_rotary_norm_bwd_bytes; dw[i] NULL = not wanted.  headdim <= 1024, rot even and >= 2, tokens times heads of both
+ * sides below 2^31, heads of both sides at most 2^20. */
 #define ISSM_ROT_INTERLEAVED 1u
 #define ISSM_ROT_BACK 2u
 typedef struct issm_rotary_args {

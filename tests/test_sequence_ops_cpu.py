@@ -192,3 +192,23 @@ def test_workspace_of_shared_rows(lib, batch, seqlen, channels):
     for back, share in ((0, 8 / 112), (1, 12 / 56)):
         assert lib.issm_gated_scan_workspace_bytes(C.byref(a), back, C.byref(need)) == 0
         assert 0 < need.value < share * size * 1.15 + rows * (128 + 5 * 512 + 256)   # (288 channels take the words of 320)
+
+
+def test_documented_sizes(lib):
+    """The last sizes that the header allows, and the first ones behind them."""
+    from dest3d_amd import _lib as L
+    need = C.c_size_t()
+    for sizes, ok in ((dict(batch=2 ** 16 - 1, seqlen=1, channels=4096), True), (dict(batch=2 ** 16, seqlen=1, channels=4096), False),
+                      (dict(batch=2 ** 22 - 1, seqlen=4 * 28, channels=1), True), (dict(batch=2 ** 22 - 1, seqlen=4 * 28 + 1, channels=1), False),
+                      (dict(batch=1, seqlen=2 ** 24 * 28 - 28, channels=64), True), (dict(batch=1, seqlen=2 ** 24 * 28 - 27, channels=64), False),
+                      (dict(batch=1, seqlen=28, channels=64 * (2 ** 22 - 1)), True), (dict(batch=1, seqlen=28, channels=64 * (2 ** 22 - 1) + 1), False)):
+        rc = lib.issm_gated_scan_workspace_bytes(C.byref(_scan(lib, **sizes)), 1, C.byref(need))
+        assert rc == (0 if ok else -2), sizes
+    a = L.RotaryArgs()
+    a.headdim, a.rot, a.heads[0], a.heads[1] = 64, 64, 3, 1
+    for batch, seqlen, ok in ((1, 2 ** 29 - 1, True), (1, 2 ** 29, False), (2 ** 15, 2 ** 14, False)):
+        a.batch, a.seqlen = batch, seqlen
+        assert lib.issm_rotary_norm_bwd_bytes(C.byref(a), C.byref(need)) == (0 if ok else -2)
+    for heads, ok in (((2 ** 20 - 1, 1), True), ((2 ** 20, 1), False)):
+        a.batch, a.seqlen, a.heads[0], a.heads[1] = 1, 2, *heads
+        assert lib.issm_rotary_norm_bwd_bytes(C.byref(a), C.byref(need)) == (0 if ok else -2)
