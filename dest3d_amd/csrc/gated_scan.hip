@@ -291,13 +291,11 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
   const bool ig = IG == 2 ? p.i != nullptr : IG == 1, nrm = NRM == 2 ? p.nrm : NRM == 1;
   const int c0 = first_channel<V>(cb * W + cg * V, p.C);
   Piece<BF, V> x[S], g[S], in[S];
-  Ids<S> ids;
   auto request = [&](int k) {
     const int t0 = k * T + tt * S;
     Rows<BF, V, S, BUF>(p.x, p.xb, p.xl, b, k, p.L, p.C, t0, c0).load(x);
     Rows<BF, V, S, BUF>(p.g, p.gb, p.gl, b, k, p.L, p.C, t0, c0).load(g);
     if (ig) Rows<BF, V, S, BUF>(p.i, p.ib, p.il, b, k, p.L, p.C, t0, c0).load(in);
-    if (SEQ) ids.load(p, b, t0);
   };
   float A[V];
   const bool all_near = decays<V>(p.A + c0, A);
@@ -309,6 +307,7 @@ __global__ __launch_bounds__(GS_THREADS, BF ? 4 : 2) void k_gscan_fwd(GScanP p) 
   auto begin = [&](Tile& q, int k, Maps<W>& m) {
     const int t0 = k * T + tt * S;
     q.k = k;
+    Ids<S> ids;
     if (SEQ) ids.load(p, b, t0);
     auto gates = [&](auto near) {
 #pragma unroll
