@@ -274,8 +274,9 @@ __global__ __launch_bounds__(256) void k_rotary(RotP p) {
   }
 }
 
-// Workgroups [0, blocks[0]) walk the queries' rows, those behind them the keys'; each leaves its sums of dw
-template <bool BF, int V, int NI, bool INTER, int NB, bool MANY>
+// Workgroups [0, blocks[0]) walk the queries' rows, those behind them the keys'; each leaves its sums of dw.  A row a lane at a time, MANY or not: two rows
+// asked for at a time leave too few waves (4096 x 4 tokens of 16 and 4 heads of 128, bf16: 52.9 us for 46.6)
+template <bool BF, int V, int NI, bool INTER, bool MANY>
 __global__ __launch_bounds__(256) void k_rotary_norm_bwd(RotP p) {
   extern __shared__ float sums[];   // (4, D)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & (p.lpr - 1), sub = lane / p.lpr;
@@ -289,60 +290,47 @@ __global__ __launch_bounds__(256) void k_rotary_norm_bwd(RotP p) {
   for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int v = 0; v < V; ++v) dw.one[i][v] = dw.two[i][v] = 0.0f;
-  const long step = (long)(MANY ? NB : 1) * tokens;
-  for (long u = ((long)block * 4 + wave) * step; u < p.tokens; u += (long)p.blocks[side] * 4 * step) {
+  for (long u = ((long)block * 4 + wave) * tokens; u < p.tokens; u += (long)p.blocks[side] * 4 * tokens) {
     Angles<V, NI> angles;
     Token token;
     if (!MANY) token = token_of(p, (unsigned)min(u + mine, (long)p.tokens - 1));
-    for (int n0 = 0; n0 < (MANY ? 1 : each); n0 += NB) {
-      Part<BF, V, NI, INTER> rx[NB], rg[NB];
-      unsigned h[NB];
-      bool there[NB];
-      Token at[NB];
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const int n = h0 + (MANY ? 0 : (n0 + j) * group);
-        const long t = u + mine + (MANY ? j * tokens : 0);
-        there[j] = n < heads && t < p.tokens;
-        h[j] = min(n, heads - 1);
-        at[j] = MANY ? token_of(p, (unsigned)min(t, (long)p.tokens - 1)) : token;
-        rx[j].load(p, p.x[side], place(at[j], h[j], p.s[side]), li);
-        rg[j].load(p, p.dy[side], place(at[j], h[j], p.ds[side]), li);
-      }
+    for (int n0 = 0; n0 < (MANY ? 1 : each); ++n0) {
+      const int n = h0 + (MANY ? 0 : n0 * group);
+      const long t = u + mine;
+      const unsigned h = min(n, heads - 1);
+      if (MANY) token = token_of(p, (unsigned)min(t, (long)p.tokens - 1));
+      const bool there = n < heads && t < p.tokens;
+      Part<BF, V, NI, INTER> rx, rg;
+      rx.load(p, p.x[side], place(token, h, p.s[side]), li);
+      rg.load(p, p.dy[side], place(token, h, p.ds[side]), li);
       if (!MANY && n0 == 0) angles.load(p, token.turn, li, -1.0f);
-      Nums<BF, V, NI, INTER> x[NB], g[NB];
-      float both[2 * NB];   // sums of x^2 and of w g x
+      Nums<BF, V, NI, INTER> x, g;
+      x.take(p, rx, li);
+      g.take(p, rg, li);
+      if (MANY) angles.load(p, token.turn, li, -1.0f);
+      angles.turn(p, g, li);
+      float both[2];   // sums of x^2 and of w g x
+      both[0] = x.dot(x);
+      float s = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        x[j].take(p, rx[j], li);
-        g[j].take(p, rg[j], li);
-        if (MANY) angles.load(p, at[j].turn, li, -1.0f);
-        angles.turn(p, g[j], li);
-        both[2 * j] = x[j].dot(x[j]);
-        float s = 0.0f;
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-            s = fmaf(g[j].one[i][v] * w.one[i][v], x[j].one[i][v], fmaf(g[j].two[i][v] * w.two[i][v], x[j].two[i][v], s));
-        both[2 * j + 1] = s;
-      }
+        for (int v = 0; v < V; ++v)
+          s = fmaf(g.one[i][v] * w.one[i][v], x.one[i][v], fmaf(g.two[i][v] * w.two[i][v], x.two[i][v], s));
+      both[1] = s;
       row_sums(both, p.lpr);
+      const float rstd = __builtin_amdgcn_rsqf(both[0] * p.inv_D + p.eps), mean = both[1] * rstd * p.inv_D;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const float rstd = __builtin_amdgcn_rsqf(both[2 * j] * p.inv_D + p.eps), mean = both[2 * j + 1] * rstd * p.inv_D;
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float x1 = x[j].one[i][v] * rstd, x2 = x[j].two[i][v] * rstd, g1 = g[j].one[i][v], g2 = g[j].two[i][v];
-            dw.one[i][v] = there[j] ? fmaf(g1, x1, dw.one[i][v]) : dw.one[i][v];
-            dw.two[i][v] = there[j] ? fmaf(g2, x2, dw.two[i][v]) : dw.two[i][v];
-            x[j].one[i][v] = rstd * fmaf(-x1, mean, g1 * w.one[i][v]);
-            x[j].two[i][v] = rstd * fmaf(-x2, mean, g2 * w.two[i][v]);
-          }
-        if (there[j]) x[j].store(p, p.y[side], ((u + mine + (MANY ? j * tokens : 0)) * heads + h[j]) * p.D, li);
-      }
+        for (int v = 0; v < V; ++v) {
+          const float x1 = x.one[i][v] * rstd, x2 = x.two[i][v] * rstd, g1 = g.one[i][v], g2 = g.two[i][v];
+          dw.one[i][v] = there ? fmaf(g1, x1, dw.one[i][v]) : dw.one[i][v];
+          dw.two[i][v] = there ? fmaf(g2, x2, dw.two[i][v]) : dw.two[i][v];
+          x.one[i][v] = rstd * fmaf(-x1, mean, g1 * w.one[i][v]);
+          x.two[i][v] = rstd * fmaf(-x2, mean, g2 * w.two[i][v]);
+        }
+      if (there) x.store(p, p.y[side], (t * heads + h) * p.D, li);
     }
   }
   // the rows of a wave, then the waves
@@ -410,7 +398,6 @@ static void launch_rows(RotP& p, hipStream_t st) {
 }
 template <bool BF, int V, int NI, bool INTER>
 static void launch_norm_bwd(RotP& p, hipStream_t st) {
-  constexpr int NB = 1;   // (4096 x 4 tokens of 16 and 4 heads of 128, bf16, 1 and 2: 46.6 and 52.9 us)
   const int rows = 64 / p.lpr;
   bool many = true;
   for (int i = 0; i < 2; ++i) {
@@ -419,8 +406,8 @@ static void launch_norm_bwd(RotP& p, hipStream_t st) {
     many = many && p.H[i] <= p.groups[i];
   }
   const unsigned blocks = p.blocks[0] + p.blocks[1], bytes = 4 * p.D * sizeof(float);
-  if (many) k_rotary_norm_bwd<BF, V, NI, INTER, NB, true><<<blocks, 256, bytes, st>>>(p);
-  else k_rotary_norm_bwd<BF, V, NI, INTER, NB, false><<<blocks, 256, bytes, st>>>(p);
+  if (many) k_rotary_norm_bwd<BF, V, NI, INTER, true><<<blocks, 256, bytes, st>>>(p);
+  else k_rotary_norm_bwd<BF, V, NI, INTER, false><<<blocks, 256, bytes, st>>>(p);
 }
 
 // V: the widest that both parts of a head, turned and not, are whole multiples of, if 64 lanes hold a row; up to 16 bytes an access forward (16384 tokens
