@@ -14,9 +14,15 @@
 // GS_CG * V = 64 channels are rows' pieces of 128 bytes in bf16: with half of that a row of
 // 131072 tokens of 2048 channels, 585 us at the time, took 715.
 //
-// Bound by bytes, and where rows are few by waiting for the states in front: bf16, 16 x 4096 tokens of 2048 channels (rows walked) 246 us forward,
-// 4.4 TB/s, and 426 backward, 4.4; 8 x 4096 (rows shared by two and three) 136 and 254, 4.0 and 3.7; 1 x 131072 (by sixteen and 24) 529, 4.1, and
-// 1126, 3.3: copies of it that did not wait took 465 and 852.  (Launches that clear the words and sum dA included.)  A copy of 1 GiB: 5.1 TB/s.
+// Bound by bytes, and where rows are few by waiting for the states in front (a copy of 1 GiB: 5.1 TB/s).  us forward and backward, with in_gate and beta,
+// calls one behind the other, their launches that clear the words and sum dA included (kernels alone, 8 x 4096 x 2048: 129 and 238):
+//   bf16, 2048 channels      all |A| < 1/4              wide decays     packed
+//   16 x 4096, walked        246, 4.4 TB/s   423, 4.4   256   449       256   522
+//   8 x 4096, by 2 and 3     139, 3.9        261, 3.6   132   256       156   278
+//   1 x 131072, by 16 and 24 527, 4.1       1115, 3.4   530  1137       584  1162    (copies that did not wait: 465 and 852)
+//   fp32, 1024 channels: 32 x 4096, walked 454, 4.7, and 780, 4.8 (packed 461 and 798); 8 x 4096, by 4 and 6, 120, 4.5, and 213, 4.4 (packed 125 and 226)
+// What the forms pay: packed ones look at the ids of each token, and shared ones spill there (gated_scan_dev.h); rows without buffers (odd widths in bf16, odd
+// addresses) have 64-bit places: 16 x 4096 x 2047 253 and 483, 8 x 4096 x 2047 180 and 339, whose shared forms spill too.
 #include "gated_scan_dev.h"
 
 // (every multiply-add is written as one: the forms of a kernel that do the same sums are to give the same bits)
@@ -754,8 +760,13 @@ static void launch_form(const GScanP& p, bool buffers, bool back, int blocks, hi
 }
 
 // Workgroups that share a row of a block of channels, of `rows` in all: as many as it takes for GS_WG a CU, forward and backward; rows enough to fill
-// the GPU twice are walked.  8 x 4096 x 2048 bf16 (256 rows) 129 and 248 us, walked 162 and 322; 16 x 4096 (512 rows) 261 and 488, walked 248
-// and 417; 1 x 131072 (32 rows) 532 and 1108, walked 4900 and 8600.
+// the GPU twice are walked.  (As many as fit in bf16.  Of the fp32 forms one fits forward, for its registers, and of some two backward; the
+// others start when those end, which costs nothing: with one and two a CU 8 x 4096 x 1024 fp32 takes 121 and 214 us for 120 and 212, 4 x 5001 x 801, packed,
+// 60 and 143 for 58 and 145, 1 x 65536 x 1024 223 and 462 for 220 and 447.)
+// us forward and backward, shared and walked: bf16, 8 x 4096 x 2048 (256 rows) 139 and 261, 173 and 339; 16 x 4096 x 2048 (512) 268 and 497, 248 and 422;
+// 1 x 131072 x 2048 (32) 522 and 1121, 4583 and 9183; fp32, 8 x 4096 x 1024 (128) 120 and 212, 180 and 363.  Just above 512 rows, where some
+// walk alone behind the others, two workgroups a row would be faster: 9 x 4096 x 3712 (522) 264 and 450, walked 333 and 668; 11 x 4096 x 4096 (704) 354 and
+// 625, 376 and 736.
 constexpr int GS_WG = 2, GS_WG_BACK = 3, GS_ROWS_WALKED = 2 * NCU;
 static int sharing(int rows, int tiles, bool back) {
   return rows >= GS_ROWS_WALKED ? 1 : max(1, min(tiles, ((back ? GS_WG_BACK : GS_WG) * NCU + rows - 1) / rows));

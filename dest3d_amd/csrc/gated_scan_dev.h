@@ -8,7 +8,8 @@ namespace issm {
 constexpr int GS_THREADS = 512, GS_CG = 16, GS_TT = (GS_THREADS - 64) / GS_CG;
 // Tokens of a thread: forward, in workgroups that share a row and in ones that walk it, and backward.  The forward leaves the states in front of
 // the backward's tiles.  (Bf16, 1 x 131072 x 2048, shared: forward 4 tokens 529 us, 2 714; backward, in an earlier form, 2 tokens 1181, 4 1231.
-// 16 x 4096 x 2048, walked: forward 2 tokens 246, 4, which spill, 355.)
+// 16 x 4096 x 2048, walked: forward 2 tokens 246, 4, which spill, 355.  The shared forward's 4 spill a little too, at four waves a SIMD: in bf16 with an
+// in_gate 5 registers, packed 20 or 29, without buffers 12 to 23; so do the shared backward's forms without buffers, 16 and 18.)
 constexpr int GS_S_SHARED = 4, GS_S_WALKED = 2, GS_S_BACK = 2, GS_TILE_BACK = GS_TT * GS_S_BACK;
 
 struct GScanP {

@@ -77,3 +77,26 @@ def test_registers_leave_room_for_the_workgroups(kernels, name, variants, regist
     for k, (r, scratch) in hit.items():
         assert r <= registers and scratch <= spilled, (k, r, scratch)
     assert sum(scratch for _, scratch in hit.values()) == spilled
+
+
+@pytest.mark.parametrize("name,variants,registers,spilled", [
+    # the recurrence forward, workgroups of eight waves: in bf16 two a CU; where workgroups share rows, four tokens a thread cost scratch with an in_gate (24
+    # bytes a lane with and without beta, packed 52 and 56) and without buffers (52, packed 80)
+    (r"k_gscan_fwd<true, 4, 4, 0, [01], (true|false), true, true>", 4, 128, 0),
+    (r"k_gscan_fwd<true, 4, 4, 1, [01], (true|false), true, true>", 4, 128, 156),
+    (r"k_gscan_fwd<true, 4, 4, 2, 2, (true|false), true, false>", 2, 128, 132),
+    (r"k_gscan_fwd<true, 4, 2, [012], [012], (true|false), false, (true|false)>", 10, 128, 0),
+    # in fp32 one
+    (r"k_gscan_fwd<false, 4, [24], [012], [012], (true|false), (true|false), (true|false)>", 20, 256, 0),
+    # backward: in bf16 three where rows are shared, without buffers by scratch (68 bytes, packed 76), and two where they are walked
+    (r"k_gscan_bwd<true, 4, 2, [01], [01], (true|false), true, true>", 8, 80, 0),
+    (r"k_gscan_bwd<true, 4, 2, 2, 2, (true|false), true, false>", 2, 80, 144),
+    (r"k_gscan_bwd<true, 4, 2, [012], [012], (true|false), false, (true|false)>", 10, 128, 0),
+    # in fp32 two
+    (r"k_gscan_bwd<false, 4, 2, [012], [012], (true|false), (true|false), (true|false)>", 20, 128, 0),
+    # fewer than four channels, and the single token
+    (r"k_gscan_(fwd|bwd)<(true|false), 1, [24], 2, 2, (true|false), (true|false), false>", 16, 80, 0),
+    (r"k_gscan_step<(true|false), (true|false), (true|false)>", 8, 64, 0),
+])
+def test_recurrence_leaves_room_for_its_workgroups(kernels, name, variants, registers, spilled):
+    test_registers_leave_room_for_the_workgroups(kernels, name, variants, registers, spilled)
