@@ -120,15 +120,15 @@ __device__ __forceinline__ void tile_map(const float (&sP)[TT][W], const float (
     P = cut || (SEQ && P < 0.0f) ? -1.0f : P * q;
   }
 }
-// What every segment starts from, in place of its H; returns the state behind them.
-template <bool SEQ, int TT, int W>
+// What every segment starts from, in place of its H; returns the state behind them.  ZEROS: a state of 0 stays 0, whatever a segment multiplies it by.
+template <bool SEQ, bool ZEROS, int TT, int W>
 __device__ __forceinline__ float tile_starts(const float (&sP)[TT][W], float (&sH)[TT][W], int w, bool back, float h) {
 #pragma unroll 8
   for (int i = 0; i < TT; ++i) {
     const int j = back ? TT - 1 - i : i;
     const float q = sP[j][w], f = sH[j][w];
     sH[j][w] = h;
-    h = SEQ && q < 0.0f ? f : fmaf(q, h, f);
+    h = (SEQ && q < 0.0f) || (ZEROS && h == 0.0f) ? f : fmaf(q, h, f);
   }
   return h;
 }
@@ -149,7 +149,7 @@ __device__ __forceinline__ bool decays(const float* from, float (&A)[V]) {
   bool near = true;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    A[v] = rate(from[v]);
+    A[v] = from[v];
     near = near && fabsf(A[v]) < GS_NEAR;
   }
   return __all(near);
@@ -256,14 +256,14 @@ __device__ __forceinline__ void chain_fwd(const GScanP& p, FwdShared<W>& sh, int
     if (on) {
       float Pt, Ht;
       tile_map<SEQ, GS_TT, W>(m.P, m.H, w, false, Pt, Ht);
-      const bool cut_off = SEQ && Pt < 0.0f, whole = cut_off || in_range(Pt, Ht);
+      const bool cut_off = SEQ && Pt < 0.0f, whole = in_range(Pt, Ht);
       if (SHARED && k > 0) {
         if (whole) tell(words + (long)k * 64, Ht, cut_off ? GS_STATE : __float_as_uint(Pt));
         carry = look.back(words + (long)k * 64, k, first);
       }
       float behind = cut_off ? Ht : fmaf(Pt, carry, Ht);
       if (SHARED && k + 1 < p.nk && whole) tell(words + (long)k * 64, behind, GS_STATE);
-      const float walked = tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, carry);
+      const float walked = __any(!whole) ? tile_starts<SEQ, true, GS_TT, W>(m.P, m.H, w, false, carry) : tile_starts<SEQ, false, GS_TT, W>(m.P, m.H, w, false, carry);
       if (!whole) {
         behind = walked;
         if (SHARED && k + 1 < p.nk) tell(words + (long)k * 64, behind, GS_STATE);
@@ -434,19 +434,21 @@ __device__ __forceinline__ void chain_bwd(const GScanP& p, BackMaps<W>& m, int c
     if (on) {
       float Pt, Ct;
       tile_map<SEQ, GS_TT, W>(m.P, m.C, w, true, Pt, Ct);
-      const bool cut_off = SEQ && Pt < 0.0f, whole = cut_off || in_range(Pt, Ct);
+      const bool cut_off = SEQ && Pt < 0.0f, whole = in_range(Pt, Ct);
       if (SHARED && o > 0) {
         if (whole) tell(words + (long)o * 64, Ct, cut_off ? GS_STATE : __float_as_uint(Pt));
         carry = look.back(words + (long)o * 64, o, first);
       }
       float behind = cut_off ? Ct : fmaf(Pt, carry, Ct);
       if (SHARED && o + 1 < p.nk && whole) tell(words + (long)o * 64, behind, GS_STATE);
-      const float walked = tile_starts<SEQ, GS_TT, W>(m.P, m.C, w, true, carry);
+      const bool zeros = __any(!whole);
+      const float walked = zeros ? tile_starts<SEQ, true, GS_TT, W>(m.P, m.C, w, true, carry) : tile_starts<SEQ, false, GS_TT, W>(m.P, m.C, w, true, carry);
       if (!whole) {
         behind = walked;
         if (SHARED && o + 1 < p.nk) tell(words + (long)o * 64, behind, GS_STATE);
       }
-      tile_starts<SEQ, GS_TT, W>(m.P, m.H, w, false, before);
+      if (zeros) tile_starts<SEQ, true, GS_TT, W>(m.P, m.H, w, false, before);
+      else tile_starts<SEQ, false, GS_TT, W>(m.P, m.H, w, false, before);
       carry = behind;
     }
     __syncthreads();
@@ -701,10 +703,7 @@ __global__ __launch_bounds__(256) void k_gscan_step(GStepP p) {
   }
   float h[4];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    h[v] = old.m[v];
-    if (!NRM) A[v] = rate(A[v]);   // (with beta, growth is NaN as it is.  Where A arrives it would be waited for alone: 512 rows of 4096 10.3 us for 9.2)
-  }
+  for (int v = 0; v < 4; ++v) h[v] = old.m[v];
   for (int r = row;;) {
 #pragma unroll
     for (int v = 0; v < 4; ++v) {

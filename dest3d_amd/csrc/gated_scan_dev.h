@@ -117,9 +117,6 @@ struct Piece {
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ex2(-LOG2E * x)); }
-// Growth that four tokens of a segment multiply within fp32 (exp(80) = 6e34); beyond it a channel is NaN, whichever form a call takes
-constexpr float GS_MOST = 20.0f;
-__device__ __forceinline__ float rate(float A) { return A > GS_MOST ? __builtin_nanf("") : A; }
 // a = exp(l) and beta = sqrt(1 - a^2).  Up to |l| = 1/4, -expm1(l) as its series: what is left out is below 2^-24 of it (l^6 / 7! = 4.8e-8).
 // NEAR: no l is beyond that (the same values, without the other form's exponential)
 constexpr float GS_NEAR = 0.25f;

@@ -20,8 +20,8 @@ def gated_scan(x, gate, A, in_gate=None, initial_states=None, seq_idx=None, norm
         initial_states: (batch, channels) or None
         seq_idx: (batch, seqlen) integer ids (compared as int32) of the sequences packed into a row, or None.  Every change of id is a cut that nothing
             passes; initial_states count as id 0, as in ISSM_chunk_scan_combined.
-        normalize: without it u_t enters as it is, and A may be positive, up to 20 (a channel with a larger one is NaN): states that grow are right as
-            long as they themselves stay within float32
+        normalize: without it u_t enters as it is, and A may be positive: states that grow are right as long as they, every decay, and what four
+            neighbouring decays multiply a state other than 0 by, stay within float32
         reverse: from the last token to the first; initial_states and the final states are then behind and before the row
     Return:
         h: (batch, seqlen, channels)  [, final_states (batch, channels) fp32]

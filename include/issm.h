@@ -730,8 +730,8 @@ int issm_pn2_three_interpolate_grad_cl(int32_t b, int32_t c, int32_t n, int32_t 
  * A state of one number for each channel, decayed by a gate and fed by the input:
  *   r = sigmoid(gate), l = A r, a = exp(l), beta = sqrt(1 - a^2) (ISSM_GS_NORMALIZE; else 1), u = sigmoid(in_gate) x (x without in_gate)
  *   h_t = a_t h_{t-1} + beta_t u_t,   y = h,   last = the state behind the last token
- * A <= 0 with ISSM_GS_NORMALIZE (a positive entry gives NaN there).  Without it A <= 20 (a larger entry gives NaN in its channel): states may grow
- * then, also by more than fp32 holds where they are small or 0 in front, and overflow where the states themselves leave fp32.  x, gate, in_gate, dy (B, L, C) in `dtype`, channels contiguous, element
+ * A <= 0 with ISSM_GS_NORMALIZE (a positive entry gives NaN there).  Without it A may be positive: states that grow are right as long as they, every
+ * decay, and what four neighbouring decays multiply a state other than 0 by, stay within fp32.  x, gate, in_gate, dy (B, L, C) in `dtype`, channels contiguous, element
  * strides of batch and token (0 repeats); y, dx, dgate, din_gate (B, L, C) contiguous in `dtype`; A, dA (C), h0, last, dlast, dh0 (B, C) fp32
  * contiguous.  seq_idx (B, L) int32 or NULL: every change of id from a token to the next cuts the recurrence, and no value passes, whatever it
  * is; h0 counts as id 0: it feeds a row whose first token has id 0 and no other.  ISSM_GS_REVERSE walks from the last token to the first ("first"
@@ -780,7 +780,7 @@ int issm_gated_scan_bwd(const issm_gated_scan_args* args);
 /* One token of `rows` sequences: x, gate, in_gate (rows, C) with element strides between rows, y (rows, C) contiguous, state (slots, C) fp32 with
  * state_stride >= C between slots, updated in place.  slots_of (rows) int32 or int64 (slots_64) names each row's slot, NULL: row r has slot r.  A row whose slot is
  * outside [0, slots) gives zeros and touches no state; rows of one slot are taken in their order, as tokens one behind the other.  The state shares no
- * memory with the others.  A as in issm_gated_scan_fwd; rows ceil(channels / 1024) < 2^23. */
+ * memory with the others.  A as in issm_gated_scan_fwd (a decay at a time); rows ceil(channels / 1024) < 2^23. */
 typedef struct issm_gated_scan_step_args {
   int32_t rows, channels;
   int64_t slots;

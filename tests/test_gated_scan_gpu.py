@@ -729,19 +729,38 @@ def test_growth_within_a_window():
     grown(got, want, 30 * step_error(l) + 370 * 2.0 ** -24)
 
 
-def test_growth_beyond_what_is_computed():
-    """A channel with A above 20 is NaN, in sequences and token by token; its neighbours are as they were."""
-    from dest3d_amd import gated_scan, gated_scan_step
-    for B, L in ((2, 300), (2, 1)):
-        d, _, _ = make(B, L, 6, torch.float32)
-        g = {k: None if v is None else v.cuda() for k, v in d.items()}
-        want = gated_scan(**g, normalize=False)
-        g["A"][3] = 20.5
-        got = gated_scan(**g, normalize=False)
-        assert torch.isnan(got[..., 3]).all() and torch.equal(got[..., [0, 1, 2, 4, 5]], want[..., [0, 1, 2, 4, 5]])
-    state = g["initial_states"].clone()
-    gated_scan_step(g["x"][:, 0], g["gate"][:, 0], g["A"], state, in_gate=g["in_gate"][:, 0], normalize=False)
-    assert torch.isnan(state[:, 3]).all() and torch.isfinite(state[:, [0, 1, 2, 4, 5]]).all()
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C,packed", [(2, 300, 24, False), (1, 1500, 7, True), (520, 200, 8, True), (520, 200, 7, False), (2, 100, 3, False)])
+def test_steep_growth_of_zeros(B, L, C, packed, dtype):
+    """Decays that four tokens multiply beyond fp32, each within it, on states and gradients of 0; smaller ones at both ends, where inputs and gradients are."""
+    d, dy, dlast = make(B, L, C, dtype, seed=C, initial=False)
+    g = torch.Generator().manual_seed(C)
+    d["A"] = 20.0 + 70.0 * torch.rand(C, generator=g)
+    gate = torch.full((B, L, C), 2.0)
+    gate[:, :20], gate[:, -20:] = -4.0, -4.0
+    d["gate"] = (gate + 0.1 * torch.rand(B, L, C, generator=g) - 0.1).to(dtype)
+    d["x"][:, :-20] = 0
+    dy[:, 20:] = 0
+    if packed:
+        d["seq_idx"] = torch.zeros(B, L, dtype=torch.int32)
+        d["seq_idx"][:, L // 2:] = 1
+    assert (d["A"] * torch.sigmoid(d["gate"].double())).max() < 88
+    l = (d["A"] * torch.sigmoid(d["gate"][:, :20].double())).max().item()
+    got, want = run(d, dy, dlast * 0, normalize=False), ref(d, dy, dlast * 0, normalize=False)
+    # (a step as above, its sigmoid's exponent of 4 rounded too)
+    grown(got, want, 20 * (step_error(l) + 4 * l * 2.0 ** -24))
+
+
+def test_steep_growth_for_a_token():
+    """A far above what all tokens together could take, behind gates that are nearly empty but for one."""
+    d, dy, dlast = make(2, 300, 12, torch.float32, in_gate=False)
+    d["A"] = torch.full((12,), 60.0)
+    d["gate"] = -30.0 + 0.3 * d["gate"]
+    d["gate"][:, 150] = 0.0
+    d["x"], d["initial_states"] = d["x"].abs(), d["initial_states"].abs()
+    got, want = run(d, dy.abs(), dlast.abs(), normalize=False), ref(d, dy.abs(), dlast.abs(), normalize=False)
+    # (sums of positive terms: 300 roundings of a state or what it passes back, the step's, and a sigmoid's exponent of 32)
+    grown(got, want, 300 * 2.0 ** -24 + step_error(30.0) + 32 * 2.0 ** -24)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
